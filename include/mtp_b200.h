@@ -308,6 +308,87 @@ int mtp_paged_kv_write(void* k_pages, void* v_pages, int dtype, const int32_t* p
                        int64_t D, int64_t start, int64_t n, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* serving from a paged cache (no counterparts in the reference)              */
+/* ------------------------------------------------------------------------- */
+
+/* RMSNorm of every query and key head and the position rotation, in one pass;
+ * with a page table also the write of the keys and values into the pool.
+ * Per head x of D values:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight   (normalise == 0: y = x * weight;
+ *                                              a NULL weight is 1)
+ *   the first rot_dim values in pairs (a, b) -> (a cos - b sin, b cos + a sin)
+ * with pairs (y[i], y[i + rot_dim/2]), or (y[2i], y[2i+1]) when interleaved,
+ * and cos/sin [max_pos, rot_dim/2] float32 at row positions[b, s].  fp32
+ * arithmetic, one rounding.
+ * q [B,S,Hq,D], k and v [B,S,Hkv,D] with element strides (sb, ss, sh) and a
+ * contiguous last dimension; dtype f32, bf16 or f16 for q, k, v, the outputs
+ * and the pools.  q_out [B,S,Hq,D].  Without a page table: k_out [B,Hkv,S,D]
+ * (the layout of tree_k and of mtp_paged_kv_write), v is not used.  With one:
+ * token s of sequence b goes to logical position start[b] + s (start [B]
+ * int32, on the device) of pools [num_pages,B,Hkv,page_size,D]; positions may
+ * be NULL (start[b] + s).  count [B] int32 (or NULL) limits the tokens of a
+ * sequence; the query rows behind them are zero and nothing else is written
+ * for them.  When two tokens of a call share a slot, the later one stays.  A
+ * position outside the tables, or a page id outside the pool, is recorded
+ * (MTP_ERR_DEVICE) and that token is not written (its query row is zero when
+ * its position has no angle). */
+int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const void* k, int64_t k_sb,
+                     int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
+                     const int32_t* positions, const float* cos, const float* sin, int64_t max_pos, int64_t rot_dim,
+                     const void* q_weight, int q_weight_dtype, const void* k_weight, int k_weight_dtype, float eps,
+                     int normalise, int interleaved, void* q_out, void* k_out, void* k_pages, void* v_pages,
+                     const int32_t* page_table, int64_t table_stride, int64_t num_pages, int64_t page_size,
+                     const int32_t* start, const int32_t* count, int64_t B, int64_t S, int64_t Hq, int64_t Hkv,
+                     int64_t D, void* stream);
+
+/* Bytes of workspace mtp_paged_window_attention needs; max_keys is the page
+ * table's width.  The workspace holds nothing between calls. */
+size_t mtp_paged_window_attention_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                            int64_t max_keys, int64_t window, int64_t sinks, int dtype,
+                                            int with_weights);
+
+/* Causal attention of the last tokens of every sequence over its paged cache,
+ * with grouped-query heads.  Sequence b holds seq_lens[b] tokens, the last
+ * q_lens[b] of which are the rows q[b, 0 .. q_lens[b]-1] (NULL: all S rows, or
+ * as many as the sequence has); row s sits at p = seq_lens[b] - q_lens[b] + s
+ * and sees key j iff j <= p and (window == 0 or j > p - window or j < sinks).
+ * q/out [B,S,Hq,D]; pools [num_pages,B,Hkv,page_size,D]; page_table
+ * [B,table_stride] int32 per token, any table (as in mtp_paged_attention);
+ * seq_lens, q_lens [B] int32 on the device.  dtype f32, bf16 or f16; D <= 256.
+ * Rows behind q_lens and rows of empty sequences are zero.  Cache positions
+ * that no row sees are not used and may hold anything, their page-table
+ * entries too; those that some row sees are finite.  Lengths outside
+ * [0, table_stride] or [0, min(S, seq_lens)] and page ids outside the pool are
+ * recorded (MTP_ERR_DEVICE).
+ * key_weights (S == 1; may be NULL) [B,Hkv,weight_ld] float32: every visible
+ * key's softmax weight, summed over the heads that share it, is added. */
+int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                               int64_t table_stride, const int32_t* seq_lens, const int32_t* q_lens, void* out,
+                               int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                               int64_t num_pages, int64_t page_size, float scale, int64_t window, int64_t sinks,
+                               float* key_weights, int64_t weight_ld, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Bytes of workspace mtp_paged_kv_evict needs (it holds nothing between calls). */
+size_t mtp_paged_kv_evict_workspace(int64_t B, int64_t H, int64_t budget);
+
+/* Cuts every sequence longer than `budget` to budget tokens, key head by key
+ * head: the first `sinks`, the last `recent` and, of the others, those with
+ * the greatest key_weights (ties: the lower position; NaN counts as the
+ * lowest).  The kept tokens keep their order and move to positions 0 ..
+ * budget-1 of the pool, their weights with them; the weights at budget ..
+ * seq_lens[b]-1 become 0.  kept [B,H,budget] int32: the positions that were
+ * kept, -1 behind the last one; new_lens [B] int32 = min(seq_lens, budget).
+ * Shorter sequences stay as they are.  The positions of a sequence own a slot
+ * each: with a table that maps two of them to one slot the rows moved there
+ * are unspecified.  Pools f32, bf16 or f16. */
+int mtp_paged_kv_evict(void* k_pages, void* v_pages, int dtype, const int32_t* page_table, int64_t table_stride,
+                       int64_t num_pages, int64_t page_size, const int32_t* seq_lens, float* key_weights,
+                       int64_t weight_ld, int32_t* kept, int32_t* new_lens, int64_t B, int64_t H, int64_t D,
+                       int64_t budget, int64_t sinks, int64_t recent, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* verification (lm_head GEMM -> argmax -> acceptance)                        */
 /* ------------------------------------------------------------------------- */
 

@@ -53,6 +53,15 @@ SIGNATURES = {
                                           _i64, _i64, _i64, _f, _f, _vp, _sz, _vp]),
     "mtp_paged_kv_write": (_i, [_vp, _vp, _i, _vp, _i64, _i64, _i64, _vp, _vp, _i, _i64, _vp, _vp, _i64, _i64,
                                 _i64, _i64, _i64, _vp]),
+    "mtp_qk_norm_rope": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i, _vp, _vp,
+                              _vp, _i64, _i64, _vp, _i, _vp, _i, _f, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                              _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "mtp_paged_window_attention_workspace": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i]),
+    "mtp_paged_window_attention": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64,
+                                        _i64, _i64, _f, _i64, _i64, _vp, _i64, _vp, _sz, _vp]),
+    "mtp_paged_kv_evict_workspace": (_sz, [_i64, _i64, _i64]),
+    "mtp_paged_kv_evict": (_i, [_vp, _vp, _i, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64,
+                                _i64, _i64, _i64, _vp, _sz, _vp]),
     "mtp_verify_workspace": (_sz, [_i64]),
     "mtp_verify_workspace_init": (_i, [_vp, _sz, _vp]),
     "mtp_fused_verify": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
@@ -170,6 +179,16 @@ def stream_handle(device: torch.device):
     if _raw_stream is not None:
         return _raw_stream(idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device: torch.device, fn, *args) -> int:
+    """fn(*args) with `device` current (the library launches on the current
+    device; the stream among the arguments belongs to `device`)."""
+    idx = device.index
+    if idx is None or idx == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(idx):
+        return fn(*args)
 
 
 # --------------------------------------------------------------------------- #

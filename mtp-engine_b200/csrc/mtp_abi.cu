@@ -1954,3 +1954,5 @@ int mtp_vocab_parallel_multi_verify(const void* hidden, int h_dtype, const void*
 }
 
 }  // extern "C"
+
+#include "mtp_abi_paged.cuh"

@@ -1,0 +1,379 @@
+// mtp_abi_paged.cuh -- C entry points of the operators that serve from a paged
+// cache: query/key norm with rotation and cache write, prompt and decode
+// attention with a window, eviction.  Included by mtp_abi.cu (argument checks,
+// plans and launches only; the kernels are in the headers named below).
+#pragma once
+
+#include "mtp_kvevict.cuh"
+#include "mtp_qknorm_rope.cuh"
+#include "mtp_splitattn.cuh"
+
+namespace {
+
+// Launch of a kernel that reads what the one before it on the stream wrote
+// (griddepcontrol.wait): its blocks are set up while that one runs out.
+template <typename Kern, typename... A>
+int launch_dependent(Kern kern, unsigned grid_x, unsigned grid_y, int threads, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid_x, grid_y, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MTP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+  MTP_LAUNCH_CHECK();
+  return MTP_OK;
+}
+
+bool pool_fits(int64_t P, int64_t B, int64_t H, int64_t ps) {
+  // rows of the pool are numbered in 32 bits (a row is D elements)
+  const double rows = (double)P * B * H * ps;
+  return rows < 2147483647.0;
+}
+
+// ---------------------------------------------------------------- norm + rotation
+template <typename T>
+int launch_rope_vec(const rope::Args& a, int lph, unsigned gx, unsigned gy, cudaStream_t s) {
+#define MTP_ROPE(L)                                                                              \
+  (a.interleaved ? rope::qk_norm_rope_kernel<T, L, true><<<dim3(gx, gy), rope::kThreads, 0, s>>>(a) \
+                 : rope::qk_norm_rope_kernel<T, L, false><<<dim3(gx, gy), rope::kThreads, 0, s>>>(a))
+  if (lph == 8) MTP_ROPE(8);
+  else if (lph == 16) MTP_ROPE(16);
+  else MTP_ROPE(32);
+#undef MTP_ROPE
+  MTP_LAUNCH_CHECK();
+  return MTP_OK;
+}
+
+// ---------------------------------------------------------------- window attention
+enum WindowPath { kPathSplit, kPathAny };
+
+struct WindowPlan {
+  WindowPath path = kPathAny;
+  int dp = 0;  // head size of the tiles
+  int row_tiles = 1, max_warps = 1, min_blocks = 1;
+  int64_t score_ld = 0;
+  size_t part_o = 0, part_ml = 0, scores = 0, row_ml = 0;  // bytes
+  size_t total() const { return part_o + part_ml + scores + row_ml + 256; }
+};
+
+// Blocks of 16 keys that a warp takes at least before another warp joins in.
+constexpr int kSplitMinBlocks = 4;
+
+WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_keys, int64_t window,
+                       int64_t sinks, int dtype, bool aligned, bool weights) {
+  WindowPlan p;
+  const int64_t G = Hq / Hkv;
+  int64_t most = max_keys;  // keys that one tile of rows sees
+  if (window > 0 && window + sinks + split::kRows < most) most = window + sinks + split::kRows;
+  if (is16bit(dtype) && aligned && D % 8 == 0 && D <= 256) {
+    p.path = kPathSplit;
+    p.dp = D <= 64 ? 64 : (D <= 128 ? 128 : 256);
+    p.row_tiles = (int)((S * G + split::kRows - 1) / split::kRows);
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const int sms = sm_count(dev >= 0 && dev < kMaxDevices ? dev : 0);
+    const int per_sm = p.dp == 64 ? 4 : (p.dp == 128 ? 2 : 1);  // by shared memory: 48, 96, 192 KB a block
+    const double blocks = (double)B * p.row_tiles * Hkv * ((most + split::kKeys - 1) / split::kKeys);
+    p.min_blocks = kSplitMinBlocks;
+    const int64_t all = (int64_t)sms * per_sm * split::kWarps;
+    const double want = blocks / p.min_blocks;
+    p.max_warps = (int)(want < 1 ? 1 : (want > (double)all ? all : (int64_t)want));
+    p.part_o = align256((size_t)p.max_warps * 2 * split::kRows * D * 4);
+    p.part_ml = align256((size_t)p.max_warps * 2 * split::kRows * 2 * 4);
+  }
+  if (weights) {
+    p.score_ld = (most + split::kKeys - 1) / split::kKeys * split::kKeys;
+    p.scores = align256((size_t)B * Hq * p.score_ld * 4);
+    p.row_ml = align256((size_t)B * Hq * 2 * 4);
+  }
+  return p;
+}
+
+template <typename T, int DP, bool MANY>
+int launch_split_inst(const split::Args& a, cudaStream_t s) {
+  static bool attr[kMaxDevices] = {};
+  int dev;
+  if (int st = current_device(&dev)) return st;
+  constexpr int smem = split::smem_bytes(DP);
+  if (int st = set_smem_once(split::split_attention_kernel<T, DP, MANY>, smem, attr, dev)) return st;
+  const unsigned grid = (unsigned)((a.max_warps + split::kWarps - 1) / split::kWarps);
+  split::split_attention_kernel<T, DP, MANY><<<grid, split::kThreads, smem, s>>>(a);
+  MTP_LAUNCH_CHECK();
+  const unsigned rows = (unsigned)((int64_t)a.B * a.row_tiles * a.Hkv * split::kRows);
+  return launch_dependent(split::split_merge_kernel<T>, rows, 1, split::kMergeWarps * 32, s, a);
+}
+
+template <typename T>
+int launch_split_t(const split::Args& a, int dp, cudaStream_t s) {
+  const bool many = a.S > 1;
+  if (dp == 64) return many ? launch_split_inst<T, 64, true>(a, s) : launch_split_inst<T, 64, false>(a, s);
+  if (dp == 128) return many ? launch_split_inst<T, 128, true>(a, s) : launch_split_inst<T, 128, false>(a, s);
+  return many ? launch_split_inst<T, 256, true>(a, s) : launch_split_inst<T, 256, false>(a, s);
+}
+
+// ---------------------------------------------------------------- eviction
+template <typename V>
+int launch_move(const evict::Args& a, int words, int lanes, cudaStream_t s) {
+  const unsigned grid = (unsigned)((int64_t)a.B * a.H * 2 * (words / lanes));
+  return launch_dependent(evict::evict_move_kernel<V>, grid, 1, evict::kMoveThreads, s, a, words, lanes);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const void* k, int64_t k_sb,
+                     int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
+                     const int32_t* positions, const float* cos, const float* sin, int64_t max_pos, int64_t rot_dim,
+                     const void* q_weight, int q_weight_dtype, const void* k_weight, int k_weight_dtype, float eps,
+                     int normalise, int interleaved, void* q_out, void* k_out, void* k_pages, void* v_pages,
+                     const int32_t* page_table, int64_t table_stride, int64_t num_pages, int64_t page_size,
+                     const int32_t* start, const int32_t* count, int64_t B, int64_t S, int64_t Hq, int64_t Hkv,
+                     int64_t D, void* stream) {
+  MTP_NVTX("mtp_qk_norm_rope");
+  const bool paged = page_table != nullptr;
+  if (B < 0 || S < 0 || Hq < 0 || Hkv < 0 || D <= 0 || max_pos < 0 || rot_dim < 0)
+    return fail(MTP_ERR_SHAPE, "bad norm/rotation sizes");
+  if (rot_dim % 2 != 0 || rot_dim > D)
+    return fail(MTP_ERR_SHAPE, "rotated size %lld is odd or above the head size %lld", (long long)rot_dim,
+                (long long)D);
+  if (paged && (page_size <= 0 || num_pages < 0 || table_stride < 0)) return fail(MTP_ERR_SHAPE, "bad page sizes");
+  if (!valid_dtype(dtype) || dtype == MTP_DTYPE_E4M3) return fail(MTP_ERR_DTYPE, "unsupported dtype %d", dtype);
+  if ((q_weight && (!valid_dtype(q_weight_dtype) || q_weight_dtype == MTP_DTYPE_E4M3)) ||
+      (k_weight && (!valid_dtype(k_weight_dtype) || k_weight_dtype == MTP_DTYPE_E4M3)))
+    return fail(MTP_ERR_DTYPE, "unsupported norm weight dtypes %d, %d", q_weight_dtype, k_weight_dtype);
+  if (B * S == 0 || Hq + Hkv == 0) return MTP_OK;
+  if ((Hq > 0 && (!q || !q_out)) || (Hkv > 0 && !k) || (rot_dim > 0 && (!cos || !sin)))
+    return fail(MTP_ERR_ARG, "null tensor pointer");
+  if (!paged && ((Hkv > 0 && !k_out) || !positions)) return fail(MTP_ERR_ARG, "null tensor pointer");
+  if (paged && (!k_pages || !v_pages || !start || (Hkv > 0 && !v))) return fail(MTP_ERR_ARG, "null tensor pointer");
+  const int64_t heads = Hq + (paged ? 2 : 1) * Hkv;
+  if (B > INT32_MAX / 2 || S > INT32_MAX / 2 || heads > INT32_MAX / 2 || D > INT32_MAX / 2 ||
+      (double)B * S * heads > 8e9)
+    return fail(MTP_ERR_SHAPE, "too many rows");
+  rope::Args a{};
+  const void* x[3] = {q, k, v};
+  const int64_t st[3][3] = {{q_sb, q_ss, q_sh}, {k_sb, k_ss, k_sh}, {v_sb, v_ss, v_sh}};
+  for (int i = 0; i < 3; ++i) {
+    a.x[i] = x[i];
+    a.sb[i] = st[i][0];
+    a.ss[i] = st[i][1];
+    a.sh[i] = st[i][2];
+  }
+  a.positions = positions;
+  a.cos = cos;
+  a.sin = sin;
+  a.max_pos = max_pos;
+  a.half = (int)(rot_dim / 2);
+  a.w[0] = q_weight;
+  a.w[1] = k_weight;
+  a.w_dtype[0] = q_weight_dtype;
+  a.w_dtype[1] = k_weight_dtype;
+  a.eps = eps;
+  a.normalise = normalise;
+  a.interleaved = interleaved;
+  a.q_out = q_out;
+  a.k_out = paged ? nullptr : k_out;
+  a.pages[0] = k_pages;
+  a.pages[1] = v_pages;
+  a.page_table = page_table;
+  a.table_stride = table_stride;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.start = paged ? start : nullptr;
+  a.count = count;
+  a.B = (int)B;
+  a.S = (int)S;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.dtype = dtype;
+  const int e16 = 16 / dtype_bytes(dtype);  // elements in 16 bytes
+  bool vec = D % 8 == 0 && D <= 256 && (interleaved ? a.half % 4 == 0 : a.half % 8 == 0) && aligned16(cos) &&
+             aligned16(sin) && aligned16(q_out) && aligned16(a.k_out);
+  for (int i = 0; i < (paged ? 3 : 2); ++i) {
+    vec &= aligned16(x[i]);
+    for (int d = 0; d < 3; ++d) vec &= st[i][d] % e16 == 0;
+  }
+  if (paged) vec &= aligned16(k_pages) && aligned16(v_pages);
+  int dev;
+  if (int r = current_device(&dev)) return r;
+  const cudaStream_t s = as_stream(stream);
+  if (!vec) {
+    const int64_t rows = B * S * heads, blocks = (rows + rope::kThreads / 32 - 1) / (rope::kThreads / 32);
+    if (blocks > INT32_MAX) return fail(MTP_ERR_SHAPE, "too many rows");
+    rope::qk_norm_rope_any_kernel<<<(unsigned)blocks, rope::kThreads, 0, s>>>(a);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+  }
+  const int lph = D <= 64 ? 8 : (D <= 128 ? 16 : 32);
+  const int groups = rope::kThreads / lph, sms = sm_count(dev);
+  // eight tokens to a block once that still fills the GPU twice, else one token and its heads over several blocks
+  a.tokens = S >= 8 && B * ((S + 7) / 8) >= 2 * sms ? 8 : 1;
+  const int64_t gx = B * ((S + a.tokens - 1) / a.tokens);
+  const int64_t most = (heads + groups / a.tokens - 1) / (groups / a.tokens);
+  int64_t gy = (2 * sms + gx - 1) / gx;
+  gy = gy < 1 ? 1 : (gy > most ? most : gy);
+  if (gx > INT32_MAX || gy > 65535) return fail(MTP_ERR_SHAPE, "too many rows");
+  if (dtype == MTP_DTYPE_F32) return launch_rope_vec<float>(a, lph, (unsigned)gx, (unsigned)gy, s);
+  if (dtype == MTP_DTYPE_BF16) return launch_rope_vec<__nv_bfloat16>(a, lph, (unsigned)gx, (unsigned)gy, s);
+  return launch_rope_vec<__half>(a, lph, (unsigned)gx, (unsigned)gy, s);
+}
+
+size_t mtp_paged_window_attention_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                            int64_t max_keys, int64_t window, int64_t sinks, int dtype,
+                                            int with_weights) {
+  if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_keys < 0 || Hq % Hkv != 0) return 256;
+  return window_plan(B, S, Hq, Hkv, D, max_keys, window, sinks, dtype, true, with_weights != 0).total();
+}
+
+int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                               int64_t table_stride, const int32_t* seq_lens, const int32_t* q_lens, void* out,
+                               int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                               int64_t num_pages, int64_t page_size, float scale, int64_t window, int64_t sinks,
+                               float* key_weights, int64_t weight_ld, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  MTP_NVTX("mtp_paged_window_attention");
+  if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || page_size <= 0 || num_pages < 0 || table_stride < 0 ||
+      window < 0 || sinks < 0)
+    return fail(MTP_ERR_SHAPE, "bad window attention sizes");
+  if (Hq % Hkv != 0) return fail(MTP_ERR_SHAPE, "Hq=%lld not a multiple of Hkv=%lld", (long long)Hq, (long long)Hkv);
+  if (D > 256) return fail(MTP_ERR_SHAPE, "head_dim %lld > 256", (long long)D);
+  if (key_weights && (S != 1 || weight_ld < table_stride))
+    return fail(MTP_ERR_SHAPE, "key weights need one query row per sequence and rows of the page table's width");
+  if (!valid_dtype(dtype) || dtype == MTP_DTYPE_E4M3) return fail(MTP_ERR_DTYPE, "unsupported dtype %d", dtype);
+  if (B * S == 0) return MTP_OK;
+  if (!q || !out || !seq_lens || (table_stride > 0 && (!page_table || !k_pages || !v_pages)))
+    return fail(MTP_ERR_ARG, "null tensor pointer");
+  if (!pool_fits(num_pages, B, Hkv, page_size)) return fail(MTP_ERR_SHAPE, "the pool has 2^31 rows or more");
+  if ((double)B * S * (Hq + 16.0 * Hkv) > 2147483647.0 || table_stride > INT32_MAX)
+    return fail(MTP_ERR_SHAPE, "too many query rows or positions");
+  const bool aligned = aligned16(q) && aligned16(out) && aligned16(k_pages) && aligned16(v_pages);
+  const WindowPlan p =
+      window_plan(B, S, Hq, Hkv, D, table_stride, window, sinks, dtype, aligned, key_weights != nullptr);
+  if (!workspace || workspace_bytes < p.total() || !aligned16(workspace))
+    return fail(MTP_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, needed", p.total());
+  const cudaStream_t s = as_stream(stream);
+  split::Args a{};
+  a.q = q;
+  a.out = out;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.page_table = page_table;
+  a.table_stride = table_stride;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.seq_lens = seq_lens;
+  a.q_lens = q_lens;
+  a.B = (int)B;
+  a.S = (int)S;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.G = (int)(Hq / Hkv);
+  a.D = (int)D;
+  a.dtype = dtype;
+  a.window = window == 0 || window > INT32_MAX ? INT32_MAX : (int)window;
+  a.sinks = window == 0 ? 0 : (int)(sinks < INT32_MAX ? sinks : INT32_MAX);
+  a.scale = scale;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.row_tiles = p.row_tiles;
+  a.max_warps = p.max_warps;
+  a.min_blocks = p.min_blocks;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float*>(ws + p.part_o);
+  if (key_weights) {
+    a.scores = reinterpret_cast<float*>(ws + p.part_o + p.part_ml);
+    a.score_ld = p.score_ld;
+    a.row_ml = reinterpret_cast<float*>(ws + p.part_o + p.part_ml + p.scores);
+    a.key_weights = key_weights;
+    a.weight_ld = weight_ld;
+  }
+  if (p.path == kPathSplit) {
+    if (int st = dtype == MTP_DTYPE_BF16 ? launch_split_t<__nv_bfloat16>(a, p.dp, s)
+                                         : launch_split_t<__half>(a, p.dp, s))
+      return st;
+  } else {
+    split::split_any_kernel<<<(unsigned)(B * S * Hq), split::kAnyWarps * 32, 0, s>>>(a);
+    MTP_LAUNCH_CHECK();
+  }
+  if (key_weights && p.score_ld > 0) {
+    const int64_t per_unit = (p.score_ld + 255) / 256;
+    return launch_dependent(split::split_key_weights_kernel, (unsigned)(B * Hkv),
+                            (unsigned)(per_unit < 65535 ? per_unit : 65535), 256, s, a);
+  }
+  return MTP_OK;
+}
+
+size_t mtp_paged_kv_evict_workspace(int64_t B, int64_t H, int64_t budget) {
+  if (B <= 0 || H <= 0 || budget <= 0) return 256;
+  return align256((size_t)B * H * budget * 8) + 256;
+}
+
+int mtp_paged_kv_evict(void* k_pages, void* v_pages, int dtype, const int32_t* page_table, int64_t table_stride,
+                       int64_t num_pages, int64_t page_size, const int32_t* seq_lens, float* key_weights,
+                       int64_t weight_ld, int32_t* kept, int32_t* new_lens, int64_t B, int64_t H, int64_t D,
+                       int64_t budget, int64_t sinks, int64_t recent, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  MTP_NVTX("mtp_paged_kv_evict");
+  if (B < 0 || H <= 0 || D <= 0 || page_size <= 0 || num_pages < 0 || table_stride < 0 || weight_ld < 0 ||
+      budget < 0 || sinks < 0 || recent < 0)
+    return fail(MTP_ERR_SHAPE, "bad eviction sizes");
+  if (sinks > budget || recent > budget - sinks)
+    return fail(MTP_ERR_SHAPE, "sinks %lld and recent %lld do not fit the budget of %lld", (long long)sinks,
+                (long long)recent, (long long)budget);
+  if (!valid_dtype(dtype) || dtype == MTP_DTYPE_E4M3) return fail(MTP_ERR_DTYPE, "unsupported dtype %d", dtype);
+  if (B == 0) return MTP_OK;
+  if (!seq_lens || !new_lens || (budget > 0 && !kept) ||
+      (table_stride > 0 && weight_ld > 0 && (!k_pages || !v_pages || !page_table || !key_weights)))
+    return fail(MTP_ERR_ARG, "null tensor pointer");
+  if (!pool_fits(num_pages, B, H, page_size)) return fail(MTP_ERR_SHAPE, "the pool has 2^31 rows or more");
+  if (table_stride > INT32_MAX || budget > INT32_MAX / 2 || (double)B * H * D * 2 > 2147483647.0)
+    return fail(MTP_ERR_SHAPE, "too many positions or heads");
+  if (!workspace || workspace_bytes < mtp_paged_kv_evict_workspace(B, H, budget) || !aligned16(workspace))
+    return fail(MTP_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, needed",
+                mtp_paged_kv_evict_workspace(B, H, budget));
+  evict::Args a{};
+  a.pages[0] = k_pages;
+  a.pages[1] = v_pages;
+  a.page_table = page_table;
+  a.table_stride = table_stride;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.seq_lens = seq_lens;
+  a.weights = key_weights;
+  a.weight_ld = weight_ld;
+  a.kept = kept;
+  a.new_lens = new_lens;
+  a.rows = static_cast<int2*>(workspace);
+  a.B = (int)B;
+  a.H = (int)H;
+  a.D = (int)D;
+  a.budget = (int)budget;
+  a.sinks = (int)sinks;
+  a.recent = (int)recent;
+  int dev;
+  if (int st = current_device(&dev)) return st;
+  const cudaStream_t s = as_stream(stream);
+  evict::evict_select_kernel<<<(unsigned)(B * H), evict::kThreads, 0, s>>>(a);
+  MTP_LAUNCH_CHECK();
+  if (budget == 0 || table_stride <= budget || weight_ld <= budget) return MTP_OK;  // no sequence is longer
+  const int row_bytes = (int)D * dtype_bytes(dtype);
+  const bool wide = row_bytes % 16 == 0 && aligned16(k_pages) && aligned16(v_pages);
+  const int word = wide ? 16 : dtype_bytes(dtype);
+  const int words = row_bytes / word;
+  // 128 bytes of a row to a block, or 32 where that leaves SMs without one
+  int lanes = 8;
+  while (words % lanes != 0) lanes >>= 1;
+  if (wide)
+    while (lanes > 2 && B * H * 2 * (words / lanes) < 2 * sm_count(dev)) lanes >>= 1;
+  if (word == 16) return launch_move<uint4>(a, words, lanes, s);
+  if (word == 4) return launch_move<uint32_t>(a, words, lanes, s);
+  return launch_move<uint16_t>(a, words, lanes, s);
+}
+
+}  // extern "C"

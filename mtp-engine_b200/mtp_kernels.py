@@ -20,6 +20,11 @@ Operators provided here (reference file:line):
   fused_causal_attention_fp8 mtp_kernels.py:1105-1133
   fused_int4_matmul          mtp_kernels.py:1194-1219
   paged_kv_write             (new: batched PagedKVCache.write_inplace, mtp_engine.py:582-586)
+  fused_qk_norm_rope / fused_qk_norm_rope_paged
+                             (new: norm and rotation of queries and keys, cache write)
+  fused_paged_prompt_attention / fused_paged_decode_attention
+                             (new: causal attention over the paged cache, windows and sinks)
+  paged_kv_evict             (new: cut the cache by accumulated attention weight)
   quantize_fp8_e4m3 / dequantize_fp8 / quantize_int4 / dequantize_int4 /
   pack_scales / unpack_scale_tensor
                              mtp_kernels.py:704-767, 1336-1353
@@ -414,6 +419,235 @@ def paged_kv_write(
         B, H, D, int(start), n, _N.stream_handle(dev)), "paged_kv_write")
 
 
+# --------------------------------------------------------------------------- #
+# serving from a paged cache: what fills it, reads it and cuts it
+# --------------------------------------------------------------------------- #
+def _i32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.contiguous().to(torch.int32)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with a contiguous last dimension (views into a fused projection's
+    output are taken as they are)."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _qk_norm_rope(q, k, v, positions, cos, sin, q_weight, k_weight, eps, interleaved, k_pages, v_pages, page_table,
+                  start, count, what):
+    q, k = _rows(q), _rows(k)
+    B, S, Hq, D = q.shape
+    Hkv = k.shape[2]
+    assert k.shape == (B, S, Hkv, D), f"q is {tuple(q.shape)}, k is {tuple(k.shape)}"
+    assert k.dtype == q.dtype
+    cos, sin = cos.contiguous(), sin.contiguous()
+    assert cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32, \
+        "cos and sin are float32 [positions, rotated / 2]"
+    if positions is not None:
+        positions = _i32(positions)
+        assert positions.shape == (B, S)
+    for w in (q_weight, k_weight):
+        assert w is None or w.shape == (D,), "norm weights must have shape [D]"
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
+    P = ps = width = 0
+    vs = (0, 0, 0)
+    if page_table is not None:
+        v = _rows(v)
+        assert v.shape == k.shape and v.dtype == q.dtype
+        assert k_pages.is_contiguous() and v_pages.is_contiguous(), "page pools are written in place"
+        P, Bp, Hp, ps, Dp = k_pages.shape
+        assert (Bp, Hp, Dp) == (B, Hkv, D) and v_pages.shape == k_pages.shape
+        assert k_pages.dtype == q.dtype and v_pages.dtype == q.dtype
+        page_table, start = _i32(page_table), _i32(start)
+        assert page_table.dim() == 2 and page_table.shape[0] == B and start.shape == (B,)
+        width, vs = page_table.shape[1], v.stride()
+        if count is not None:
+            count = _i32(count)
+            assert count.shape == (B,)
+    dev = _N.require_cuda(q, k, v if page_table is not None else None, positions, cos, sin, q_weight, k_weight,
+                          k_pages, v_pages, page_table, start, count)
+    q_out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=q.device)
+    k_out = None if page_table is not None else torch.empty((B, Hkv, S, D), dtype=q.dtype, device=q.device)
+    qs, ks = q.stride(), k.stride()
+    ptr, code = _N.ptr, _N.dtype_code
+    _N.check(_N.call_on(
+        dev, _N.lib().mtp_qk_norm_rope, ptr(q), qs[0], qs[1], qs[2], ptr(k), ks[0], ks[1], ks[2],
+        ptr(v) if page_table is not None else None, vs[0], vs[1], vs[2], code(q), ptr(positions), ptr(cos), ptr(sin),
+        cos.shape[0], 2 * cos.shape[1], ptr(q_weight), 0 if q_weight is None else code(q_weight), ptr(k_weight),
+        0 if k_weight is None else code(k_weight), 0.0 if eps is None else float(eps), int(eps is not None),
+        int(interleaved), ptr(q_out), ptr(k_out), ptr(k_pages), ptr(v_pages), ptr(page_table), width, P, ps,
+        ptr(start), ptr(count), B, S, Hq, Hkv, D, _N.stream_handle(dev)), what)
+    return q_out, k_out
+
+
+def fused_qk_norm_rope(
+    q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+    q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+    eps: Optional[float] = 1e-6, *, interleaved: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every query and key head and their position rotation, in one
+    pass (fp32 inside, rounded once).
+
+    q [B,S,Hq,D], k [B,S,Hkv,D] (any strides with a contiguous last dimension,
+    e.g. slices of a fused projection's output); positions [B,S] int; cos/sin
+    [max_pos, R/2] float32, R <= D: the first R values of a head turn, in
+    pairs (i, i + R/2), or (2i, 2i + 1) when ``interleaved``.  q_weight /
+    k_weight [D] are the norms' gammas; eps=None leaves the norm out.
+    Returns q [B,S,Hq,D] and k [B,Hkv,S,D], the layouts that
+    ``fused_tree_attention_paged`` (tree nodes at their depth's position) and
+    ``paged_kv_write`` take.  A position outside the tables gives zero rows
+    and is recorded (``device_status``)."""
+    assert positions is not None
+    return _qk_norm_rope(q, k, None, positions, cos, sin, q_weight, k_weight, eps, interleaved, None, None, None,
+                         None, None, "fused_qk_norm_rope")
+
+
+def fused_qk_norm_rope_paged(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor], cos: torch.Tensor,
+    sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
+    q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+    eps: Optional[float] = 1e-6, *, count: Optional[torch.Tensor] = None, interleaved: bool = False,
+) -> torch.Tensor:
+    """``fused_qk_norm_rope`` that writes the keys, and the values v
+    [B,S,Hkv,D], straight into a PagedKVCache pool: token s of sequence b goes
+    to logical position start[b] + s (start [B] int, on the device) of
+    k/v_pages [P,B,Hkv,page_size,D] (written in place, contiguous) through
+    page_table [B,L] (per token).  positions=None rotates by start[b] + s;
+    after an eviction a token's position and its place in the cache differ.
+    count [B] limits the tokens of each sequence: the rows behind them are
+    zero in the returned q [B,S,Hq,D] and touch nothing in the pool.  When two
+    tokens of one call map to one slot, the later stays."""
+    return _qk_norm_rope(q, k, v, positions, cos, sin, q_weight, k_weight, eps, interleaved, k_pages, v_pages,
+                         page_table, start, count, "fused_qk_norm_rope_paged")[0]
+
+
+def _window_attention(q4, out, k_pages, v_pages, page_table, seq_lens, q_lens, scale, window, sinks, key_weights,
+                      what):
+    B, S, Hq, D = q4
+    P, Bp, Hkv, ps, Dp = k_pages.shape
+    assert (Bp, Dp) == (B, D) and v_pages.shape == k_pages.shape
+    assert k_pages.dtype == out.dtype and v_pages.dtype == out.dtype
+    assert Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}"
+    assert page_table.dim() == 2 and page_table.shape[0] == B and seq_lens.shape == (B,)
+    assert window is None or window > 0, "window is a positive number of positions, or None"
+    assert sinks >= 0
+    width = page_table.shape[1]
+    weight_ld = 0
+    if key_weights is not None:
+        assert key_weights.dtype == torch.float32 and key_weights.is_contiguous(), "key_weights is added to in place"
+        assert key_weights.shape[:2] == (B, Hkv) and key_weights.dim() == 3 and key_weights.shape[2] >= width
+        weight_ld = key_weights.shape[2]
+    return B, S, Hq, Hkv, D, P, ps, width, weight_ld, (1.0 / math.sqrt(D) if scale is None else float(scale)), \
+        (0 if window is None else int(window))
+
+
+def _run_window_attention(q, out, k_pages, v_pages, page_table, seq_lens, q_lens, dims, sinks, key_weights, dev, what):
+    B, S, Hq, Hkv, D, P, ps, width, weight_ld, scale, window = dims
+    L, ptr, code = _N.lib(), _N.ptr, _N.dtype_code(q)
+    # scratch of this call alone: nothing is kept, and captured graphs share none
+    nbytes = _N.call_on(dev, L.mtp_paged_window_attention_workspace, B, S, Hq, Hkv, D, width, window, sinks, code,
+                        int(key_weights is not None))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _N.check(_N.call_on(
+        dev, L.mtp_paged_window_attention, ptr(q), ptr(k_pages), ptr(v_pages), ptr(page_table), width, ptr(seq_lens),
+        ptr(q_lens), ptr(out), code, B, S, Hq, Hkv, D, P, ps, scale, window, sinks, ptr(key_weights), weight_ld,
+        ptr(ws), nbytes, _N.stream_handle(dev)), what)
+    return out
+
+
+def fused_paged_prompt_attention(
+    q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+    seq_lens: torch.Tensor, q_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None, *,
+    window: Optional[int] = None, sinks: int = 0,
+) -> torch.Tensor:
+    """Causal attention of a prompt (or of a piece of one, behind tokens that
+    are cached already) over a PagedKVCache pool, with grouped-query heads.
+
+    q [B,S,Hq,D]; k/v_pages [P,B,Hkv,page_size,D]; page_table [B,L] per-token
+    page ids (any table); seq_lens [B] int: tokens in the cache, the new ones
+    included; q_lens [B] int: new tokens of each sequence, the last q_lens[b]
+    of it (None: all S rows).  Row s < q_lens[b] sits at position
+    p = seq_lens[b] - q_lens[b] + s and sees key j iff j <= p and, with a
+    ``window``, p - j < window or j < ``sinks``.  Returns [B,S,Hq,D] in q.dtype;
+    rows behind q_lens are zero.  Cache positions that no row of the call sees
+    may hold anything, their page-table entries too."""
+    q, k_pages, v_pages = q.contiguous(), k_pages.contiguous(), v_pages.contiguous()
+    page_table, seq_lens = _i32(page_table), _i32(seq_lens)
+    if q_lens is not None:
+        q_lens = _i32(q_lens)
+        assert q_lens.shape == (q.shape[0],)
+    dims = _window_attention(q.shape, q, k_pages, v_pages, page_table, seq_lens, q_lens, scale, window, sinks, None,
+                             "fused_paged_prompt_attention")
+    dev = _N.require_cuda(q, k_pages, v_pages, page_table, seq_lens, q_lens)
+    return _run_window_attention(q, torch.empty_like(q), k_pages, v_pages, page_table, seq_lens, q_lens, dims, sinks,
+                                 None, dev, "fused_paged_prompt_attention")
+
+
+def fused_paged_decode_attention(
+    q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+    seq_lens: torch.Tensor, scale: Optional[float] = None, *,
+    window: Optional[int] = None, sinks: int = 0, key_weights: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of one new token per sequence over a PagedKVCache pool, with
+    grouped-query heads and ragged lengths; long caches are split over the GPU.
+
+    q [B,Hq,D]; pools, page_table, window and sinks as in
+    ``fused_paged_prompt_attention``; seq_lens [B] int (the new token
+    included; an empty sequence gives zero rows).  key_weights [B,Hkv,>=L]
+    float32 (optional): every visible key's softmax weight, summed over the
+    query heads that share it, is added in place -- the totals that
+    ``paged_kv_evict`` goes by.  Returns [B,Hq,D] in q.dtype."""
+    q, k_pages, v_pages = q.contiguous(), k_pages.contiguous(), v_pages.contiguous()
+    page_table, seq_lens = _i32(page_table), _i32(seq_lens)
+    B, Hq, D = q.shape
+    dims = _window_attention((B, 1, Hq, D), q, k_pages, v_pages, page_table, seq_lens, None, scale, window, sinks,
+                             key_weights, "fused_paged_decode_attention")
+    dev = _N.require_cuda(q, k_pages, v_pages, page_table, seq_lens, key_weights)
+    return _run_window_attention(q, torch.empty_like(q), k_pages, v_pages, page_table, seq_lens, None, dims, sinks,
+                                 key_weights, dev, "fused_paged_decode_attention")
+
+
+def paged_kv_evict(
+    k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+    key_weights: torch.Tensor, budget: int, *, sinks: int = 0, recent: int = 0,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cut every sequence longer than ``budget`` to budget tokens, in place and
+    key head by key head: the first ``sinks``, the last ``recent`` and, of the
+    others, those with the greatest ``key_weights`` [B,Hkv,>=L] float32 (ties:
+    the lower position; NaN counts as the lowest).
+
+    The kept tokens keep their order and move to positions 0 .. budget-1 of
+    k/v_pages [P,B,Hkv,page_size,D] through page_table [B,L] (whose positions
+    own a slot each), their weights with them; the weights behind them become
+    0.  Returns (kept [B,Hkv,budget] int32: the positions that stayed, -1
+    behind the last; new_lens [B] int32).  The pages behind new_lens are free.
+    Keys in the cache carry their rotation, so a new token still rotates by
+    its own position (``fused_qk_norm_rope_paged``: positions and start)."""
+    assert k_pages.is_contiguous() and v_pages.is_contiguous(), "page pools are changed in place"
+    assert key_weights.dtype == torch.float32 and key_weights.is_contiguous(), "key_weights is changed in place"
+    P, B, Hkv, ps, D = k_pages.shape
+    assert v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype
+    page_table, seq_lens = _i32(page_table), _i32(seq_lens)
+    assert page_table.dim() == 2 and page_table.shape[0] == B and seq_lens.shape == (B,)
+    assert key_weights.dim() == 3 and key_weights.shape[:2] == (B, Hkv)
+    assert key_weights.shape[2] >= page_table.shape[1]
+    assert budget >= 0 and sinks >= 0 and recent >= 0 and sinks + recent <= budget, \
+        f"sinks={sinks} and recent={recent} do not fit budget={budget}"
+    dev = _N.require_cuda(k_pages, v_pages, page_table, seq_lens, key_weights)
+    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
+    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    L, ptr = _N.lib(), _N.ptr
+    nbytes = L.mtp_paged_kv_evict_workspace(B, Hkv, budget)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _N.check(_N.call_on(
+        dev, L.mtp_paged_kv_evict, ptr(k_pages), ptr(v_pages), _N.dtype_code(k_pages), ptr(page_table),
+        page_table.shape[1], P, ps, ptr(seq_lens), ptr(key_weights), key_weights.shape[2], ptr(kept), ptr(new_lens),
+        B, Hkv, D, int(budget), int(sinks), int(recent), ptr(ws), nbytes, _N.stream_handle(dev)), "paged_kv_evict")
+    return kept, new_lens
+
+
 def fused_int4_matmul(
     x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, K: int, group: int = 32,
 ) -> torch.Tensor:
@@ -552,6 +786,8 @@ __all__ = [
     "fused_rmsnorm_linear", "fused_rmsnorm_linear_fp8",
     "fused_tree_attention", "fused_paged_attention", "fused_tree_attention_paged",
     "fused_tree_attn_rmsnorm_linear", "paged_kv_write",
+    "fused_qk_norm_rope", "fused_qk_norm_rope_paged", "fused_paged_prompt_attention",
+    "fused_paged_decode_attention", "paged_kv_evict",
     "fused_causal_attention", "fused_causal_attention_fp8", "fused_int4_matmul", "quantize_int4", "dequantize_int4",
     "quantize_fp8_e4m3", "quantize_fp8_rows", "dequantize_fp8", "pack_scales", "unpack_scale_tensor",
     "_HAS_TRITON",
