@@ -5,6 +5,7 @@
 #pragma once
 
 #include "mtp_kvevict.cuh"
+#include "mtp_promptattn_tc.cuh"
 #include "mtp_qknorm_rope.cuh"
 #include "mtp_splitattn.cuh"
 
@@ -49,12 +50,14 @@ int launch_rope_vec(const rope::Args& a, int lph, unsigned gx, unsigned gy, cuda
 }
 
 // ---------------------------------------------------------------- window attention
-enum WindowPath { kPathSplit, kPathAny };
+enum WindowPath { kPathTensor, kPathSplit, kPathAny };
+constexpr int kNoWindow = 1 << 30;  // positions stay below it, so differences of positions fit 32 bits
 
 struct WindowPlan {
   WindowPath path = kPathAny;
   int dp = 0;  // head size of the tiles
   int row_tiles = 1, max_warps = 1, min_blocks = 1;
+  int tpt = 0, pairs = 0, splits = 1;  // tensor-core tiles
   int64_t score_ld = 0;
   size_t part_o = 0, part_ml = 0, scores = 0, row_ml = 0;  // bytes
   size_t total() const { return part_o + part_ml + scores + row_ml + 256; }
@@ -63,19 +66,53 @@ struct WindowPlan {
 // Blocks of 16 keys that a warp takes at least before another warp joins in.
 constexpr int kSplitMinBlocks = 4;
 
+// Which kernel, from types, sizes and alignment alone:
+//   16-bit, head sizes 64 .. 128 in steps of 8, more than 16 rows per key head: tcgen05 tiles;
+//   other 16-bit calls with head sizes up to 256 in steps of 8: warp-level tiles of 16 rows;
+//   everything else: one block per row, fp32.
 WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_keys, int64_t window,
                        int64_t sinks, int dtype, bool aligned, bool weights) {
   WindowPlan p;
   const int64_t G = Hq / Hkv;
-  int64_t most = max_keys;  // keys that one tile of rows sees
-  if (window > 0 && window + sinks + split::kRows < most) most = window + sinks + split::kRows;
-  if (is16bit(dtype) && aligned && D % 8 == 0 && D <= 256) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int sms = sm_count(dev >= 0 && dev < kMaxDevices ? dev : 0);
+  const bool wide = is16bit(dtype) && aligned && D % 8 == 0 && D <= 256;
+  if (wide && D >= 64 && D <= 128 && S > 1 && S * G > split::kRows && G <= 128) {
+    p.path = kPathTensor;
+    p.dp = D <= 64 ? 64 : 128;
+    p.tpt = (int)(128 / G);
+    p.pairs = (int)((S + 2 * p.tpt - 1) / (2 * p.tpt));
+    const double items = (double)B * Hkv * p.pairs;
+    int64_t most = max_keys;
+    if (window > 0 && window + sinks + 2 * p.tpt < most) most = window + sinks + 2 * p.tpt;
+    const int64_t chunks = most / attn::kChunk + 1;
+    // Fewer items than SMs, or a last round that leaves most of them idle: cut
+    // the chunk lists.  Cost in chunks: a round is one piece and about 1.5
+    // chunks of set-up and output; joining the pieces costs about 3.
+    double best = 0;
+    for (int n = 1; n <= 32 && n * 2 <= chunks + 1; ++n) {
+      if (n > 1 && items * n > 8.0 * sms) break;
+      const double rounds = (double)(int64_t)((items * n + sms - 1) / sms);
+      const double cost = rounds * ((double)chunks / n + 1.5) + (n > 1 ? 3.0 : 0.0);
+      if (n == 1 || cost < best) {
+        best = cost;
+        p.splits = n;
+      }
+    }
+    if (p.splits > 1) {
+      const size_t slots = (size_t)B * Hkv * p.pairs * p.splits * 256;
+      p.part_o = align256(slots * D * 4);
+      p.part_ml = align256(slots * 2 * 4);
+    }
+    return p;
+  }
+  if (wide) {
+    int64_t most = max_keys;  // keys that one tile of rows sees
+    if (window > 0 && window + sinks + split::kRows < most) most = window + sinks + split::kRows;
     p.path = kPathSplit;
     p.dp = D <= 64 ? 64 : (D <= 128 ? 128 : 256);
     p.row_tiles = (int)((S * G + split::kRows - 1) / split::kRows);
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const int sms = sm_count(dev >= 0 && dev < kMaxDevices ? dev : 0);
     const int per_sm = p.dp == 64 ? 4 : (p.dp == 128 ? 2 : 1);  // by shared memory: 48, 96, 192 KB a block
     const double blocks = (double)B * p.row_tiles * Hkv * ((most + split::kKeys - 1) / split::kKeys);
     p.min_blocks = kSplitMinBlocks;
@@ -86,11 +123,97 @@ WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
     p.part_ml = align256((size_t)p.max_warps * 2 * split::kRows * 2 * 4);
   }
   if (weights) {
-    p.score_ld = (most + split::kKeys - 1) / split::kKeys * split::kKeys;
+    p.score_ld = (max_keys + split::kKeys - 1) / split::kKeys * split::kKeys;
+    if (window > 0 && window + sinks + split::kKeys < p.score_ld)
+      p.score_ld = (window + sinks + split::kKeys) / split::kKeys * split::kKeys;
     p.scores = align256((size_t)B * Hq * p.score_ld * 4);
     p.row_ml = align256((size_t)B * Hq * 2 * 4);
   }
   return p;
+}
+
+template <int AB_FMT, int DP>
+int launch_prompt_inst(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const prompt::Params& p,
+                       int sms, int dev, cudaStream_t s) {
+  static bool attr[kMaxDevices] = {};
+  static bool regs_ok[kMaxDevices] = {};
+  constexpr int smem = prompt::smem_bytes(DP);
+  if (!regs_ok[dev]) {  // setmaxnreg moves registers inside the launch's reservation; with another one it could wait
+    cudaFuncAttributes fa;
+    MTP_CUDA_TRY(cudaFuncGetAttributes(&fa, prompt::prompt_attention_tc_kernel<AB_FMT, DP>));
+    if (fa.numRegs != prompt::kLaunchRegs)
+      return fail(MTP_ERR_CUDA, "prompt attention kernel reserves %d registers per thread, its register split needs %d",
+                  fa.numRegs, prompt::kLaunchRegs);
+    regs_ok[dev] = true;
+  }
+  if (int st = set_smem_once(prompt::prompt_attention_tc_kernel<AB_FMT, DP>, smem, attr, dev)) return st;
+  const unsigned grid = (unsigned)(p.items < sms ? p.items : sms);
+  prompt::prompt_attention_tc_kernel<AB_FMT, DP><<<grid, prompt::kThreads, smem, s>>>(tq, tk, tv, p);
+  MTP_LAUNCH_CHECK();
+  if (p.splits == 1) return MTP_OK;
+  const int64_t warps = (int64_t)p.B * p.S * p.Hq;
+  return launch_dependent(prompt::prompt_merge_kernel<typename std::conditional<AB_FMT == 1, __nv_bfloat16, __half>::type>,
+                          (unsigned)((warps + 7) / 8), 1, 256, s, p);
+}
+
+int launch_prompt(const split::Args& a, const WindowPlan& pl, cudaStream_t s) {
+  const int ps = (int)a.page_size;
+  prompt::Params p{};
+  p.slab = ps % attn::kChunk == 0 ? attn::kChunk
+                                  : (ps >= 8 && attn::kChunk % ps == 0 ? ps : 0);
+  const uint64_t D = a.D, E = 2;
+  CUtensorMap tq, tk, tv;
+  {
+    const uint64_t dims[4] = {D, (uint64_t)a.Hq, (uint64_t)a.S, (uint64_t)a.B};
+    const uint64_t str[3] = {D * E, (uint64_t)a.Hq * D * E, (uint64_t)a.S * a.Hq * D * E};
+    const uint32_t box[4] = {64, (uint32_t)a.G, (uint32_t)pl.tpt, 1};
+    if (int st = make_map(&tq, a.q, a.dtype, 4, dims, str, box)) return st;
+  }
+  {
+    // pools as [P * B * Hkv * page_size, D]: one (page, b, h) slab = page_size consecutive rows
+    const uint64_t rows = (uint64_t)a.num_pages * a.B * a.Hkv * ps;
+    const uint64_t dims[2] = {D, rows > 0 ? rows : 1};
+    const uint64_t str[1] = {D * E};
+    const uint32_t box[2] = {64, (uint32_t)(p.slab > 0 ? p.slab : 8)};
+    const void* k = rows > 0 ? a.k_pages : a.q;  // an empty pool is never read
+    const void* v = rows > 0 ? a.v_pages : a.q;
+    if (int st = make_map(&tk, k, a.dtype, 2, dims, str, box)) return st;
+    if (int st = make_map(&tv, v, a.dtype, 2, dims, str, box)) return st;
+  }
+  p.page_table = a.page_table;
+  p.table_stride = a.table_stride;
+  p.k_pool = static_cast<const uint8_t*>(a.k_pages);
+  p.v_pool = static_cast<const uint8_t*>(a.v_pages);
+  p.seq_lens = a.seq_lens;
+  p.q_lens = a.q_lens;
+  p.out = a.out;
+  p.part_o = a.part_o;
+  p.part_ml = a.part_ml;
+  p.B = a.B;
+  p.S = a.S;
+  p.Hq = a.Hq;
+  p.Hkv = a.Hkv;
+  p.G = a.G;
+  p.D = a.D;
+  p.ps = ps;
+  p.num_pages = (int)a.num_pages;
+  p.window = a.window;
+  p.sinks = a.sinks;
+  p.tpt = pl.tpt;
+  p.pairs = pl.pairs;
+  p.splits = pl.splits;
+  p.items = a.B * a.Hkv * pl.pairs * pl.splits;
+  p.table_vec = aligned16(a.page_table) && a.table_stride % 4 == 0;
+  p.dtype = a.dtype;
+  p.scale_log2 = a.scale_log2;
+  int dev;
+  if (int st = current_device(&dev)) return st;
+  const int sms = sm_count(dev);
+  if (a.dtype == MTP_DTYPE_BF16)
+    return pl.dp == 64 ? launch_prompt_inst<1, 64>(tq, tk, tv, p, sms, dev, s)
+                       : launch_prompt_inst<1, 128>(tq, tk, tv, p, sms, dev, s);
+  return pl.dp == 64 ? launch_prompt_inst<0, 64>(tq, tk, tv, p, sms, dev, s)
+                     : launch_prompt_inst<0, 128>(tq, tk, tv, p, sms, dev, s);
 }
 
 template <typename T, int DP, bool MANY>
@@ -250,9 +373,11 @@ int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v
   if (!q || !out || !seq_lens || (table_stride > 0 && (!page_table || !k_pages || !v_pages)))
     return fail(MTP_ERR_ARG, "null tensor pointer");
   if (!pool_fits(num_pages, B, Hkv, page_size)) return fail(MTP_ERR_SHAPE, "the pool has 2^31 rows or more");
-  if ((double)B * S * (Hq + 16.0 * Hkv) > 2147483647.0 || table_stride > INT32_MAX)
+  if ((double)B * S * (Hq + 16.0 * Hkv) > 2147483647.0 || table_stride > kNoWindow || num_pages > INT32_MAX ||
+      page_size > INT32_MAX)
     return fail(MTP_ERR_SHAPE, "too many query rows or positions");
-  const bool aligned = aligned16(q) && aligned16(out) && aligned16(k_pages) && aligned16(v_pages);
+  // the tiles fold a positive scale into the exponent
+  const bool aligned = aligned16(q) && aligned16(out) && aligned16(k_pages) && aligned16(v_pages) && scale > 0.f;
   const WindowPlan p =
       window_plan(B, S, Hq, Hkv, D, table_stride, window, sinks, dtype, aligned, key_weights != nullptr);
   if (!workspace || workspace_bytes < p.total() || !aligned16(workspace))
@@ -276,8 +401,8 @@ int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v
   a.G = (int)(Hq / Hkv);
   a.D = (int)D;
   a.dtype = dtype;
-  a.window = window == 0 || window > INT32_MAX ? INT32_MAX : (int)window;
-  a.sinks = window == 0 ? 0 : (int)(sinks < INT32_MAX ? sinks : INT32_MAX);
+  a.window = window == 0 || window > kNoWindow ? kNoWindow : (int)window;
+  a.sinks = window == 0 ? 0 : (int)(sinks < kNoWindow ? sinks : kNoWindow);
   a.scale = scale;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.row_tiles = p.row_tiles;
@@ -293,6 +418,7 @@ int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v
     a.key_weights = key_weights;
     a.weight_ld = weight_ld;
   }
+  if (p.path == kPathTensor) return launch_prompt(a, p, s);
   if (p.path == kPathSplit) {
     if (int st = dtype == MTP_DTYPE_BF16 ? launch_split_t<__nv_bfloat16>(a, p.dp, s)
                                          : launch_split_t<__half>(a, p.dp, s))

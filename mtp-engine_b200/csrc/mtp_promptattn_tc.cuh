@@ -1,0 +1,665 @@
+// mtp_promptattn_tc.cuh -- causal attention of many new tokens over a paged
+// cache (prompts, pieces of prompts) on the sm_100a tensor cores, with
+// grouped-query heads, ragged lengths, a sliding window and first tokens that
+// stay visible ("sinks").  The row and key sets are those of mtp_splitattn.cuh,
+// which serves calls with few rows.
+//
+// An item is one (sequence, key head, pair of query tiles): a tile holds
+// tpt = 128 / G positions x G heads (row r = position * G + head), so a
+// 128-key chunk of K and V is read once for 256 rows.  Persistent: one block
+// of 384 threads per SM walks over the items, the ones with the most keys
+// first and every other round in reverse, which evens out causal lengths
+// without a counter in memory.  Roles as in tree_attention_tc_kernel, whose
+// inner loop this shares:
+//   warps 0-3, 4-7  softmax of tile 0 / 1, one row per thread: scores from
+//                   tensor memory, running maximum with lazy rescaling, P
+//                   (16-bit) back over the scores' first columns, the output
+//   warp 8          producer: Q of the item, then the chunks' K and V -- whole
+//                   page slabs by TMA, or token by token where a chunk's
+//                   table is not page-granular or where the chunk holds keys
+//                   that no row of the call may see (those are zero-filled:
+//                   their slots may hold anything, and 0 * NaN is NaN)
+//   warp 9          tcgen05.mma issuer
+//   warp 10         page-table reader, up to kIdRing chunks ahead
+// All rings and barrier phases run on from item to item: the next item's keys
+// are already on their way, and its first scores are computed, while the
+// softmax warps write the last item's output.
+//
+// Chunks of an item: those that hold sinks, then those from the first row's
+// window to the last row's position; a tile stops at its own last chunk.
+//
+// Bound: the two products of a chunk take 2 x 512 tensor cycles per tile
+// (D = 128) and its 16384 exponentials 1024 cycles of the SM's exp2 units, so
+// 2048 cycles per chunk for both tiles is the floor of either pipe.
+#pragma once
+
+#include "mtp_attention_tc.cuh"
+#include "mtp_splitattn.cuh"
+
+namespace mtp {
+namespace prompt {
+
+using attn::kChunk;
+using attn::kIdRing;
+using attn::kLaunchRegs;
+using attn::kMaxPagesPerChunk;
+using attn::kRegsAux;
+using attn::kRegsSoftmax;
+using attn::kThreads;
+constexpr int kHalfBytes = 128 * 128;  // 128 rows x 64 dims
+constexpr int kWarpProducer = 8, kWarpMma = 9, kWarpTable = 10;
+constexpr int tile_bytes(int dp) { return dp / 64 * kHalfBytes; }
+constexpr int num_buf(int dp) { return dp == 128 ? 5 : 10; }  // 160 KB of K and V in flight
+constexpr int smem_bytes(int dp) {
+  return 2 * tile_bytes(dp) + num_buf(dp) * tile_bytes(dp) + kIdRing * kMaxPagesPerChunk * 4 + 512 + 1024;
+}
+static_assert(smem_bytes(128) <= 227 * 1024 && smem_bytes(64) <= 227 * 1024, "shared memory per CTA");
+
+struct Params {
+  const int32_t* page_table;
+  int64_t table_stride;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;
+  void* out;      // [B, S, Hq, D]
+  float* part_o;  // [items][256][D] (splits > 1)
+  float* part_ml; // [items][256][2]
+  int B, S, Hq, Hkv, G, D, ps, num_pages;
+  int window, sinks;
+  int slab;      // rows of a TMA page load (0: always token by token)
+  int tpt;       // positions per tile
+  int pairs;     // tile pairs per sequence
+  int splits;    // pieces of a pair's chunk list
+  int items;     // B * Hkv * pairs * splits
+  int table_vec; // page-table rows 16-byte aligned
+  int dtype;
+  float scale_log2;
+};
+
+// One item: its rows and the chunks it goes over.
+struct Item {
+  int b, kvh, s0;  // first position (row of the call) of the pair
+  int len, n;      // the sequence
+  int call_lo;     // first key that some row's window reaches
+  int ns, c_lo;    // chunks 0 .. ns-1 (sinks), then c_lo, c_lo + 1, ...
+  int i0;          // this item's part of the list: [i0, i0 + max(n_it))
+  int n_it[2];     // chunks of tile 0 and 1
+  __device__ __forceinline__ int chunk(int i) const { return i0 + i < ns ? i0 + i : c_lo + (i0 + i - ns); }
+  __device__ __forceinline__ int count() const { return max(n_it[0], n_it[1]); }
+  // whether key j may be seen by some row of the call
+  __device__ __forceinline__ bool used(const Params& p, int j) const {
+    return j < len && (j >= call_lo || j < p.sinks);
+  }
+  // whether all keys of chunk c are used
+  __device__ __forceinline__ bool whole(const Params& p, int c) const {
+    const int first = c * kChunk;
+    return first + kChunk <= len && (first >= call_lo || first + kChunk <= p.sinks);
+  }
+};
+
+__device__ __forceinline__ Item item_of(const Params& p, int index) {
+  Item it;
+  const int split = index % p.splits;
+  int u = index / p.splits;
+  it.kvh = u % p.Hkv;
+  u /= p.Hkv;
+  it.b = u % p.B;
+  it.s0 = (p.pairs - 1 - u / p.B) * 2 * p.tpt;  // the last positions first
+  const int cap = (int)min(p.table_stride, (int64_t)INT32_MAX);
+  it.len = max(0, min(__ldg(p.seq_lens + it.b), cap));
+  const int n = p.q_lens ? __ldg(p.q_lens + it.b) : p.S;
+  it.n = max(0, min(n, min(p.S, it.len)));
+  it.ns = it.c_lo = it.i0 = it.n_it[0] = it.n_it[1] = 0;
+  it.call_lo = max(0, it.len - it.n - p.window + 1);
+  if (it.s0 >= it.n) return it;
+  const int past = it.len - it.n;
+  const int lo = max(0, past + it.s0 - p.window + 1);
+  it.ns = (min(p.sinks, lo) + kChunk - 1) / kChunk;
+  it.c_lo = max(it.ns, lo / kChunk);
+  const int last0 = past + min(it.s0 + p.tpt, it.n) - 1;
+  const int e0 = it.ns + max(0, last0 / kChunk - it.c_lo + 1);
+  int e1 = 0;
+  if (it.s0 + p.tpt < it.n) {
+    const int last1 = past + min(it.s0 + 2 * p.tpt, it.n) - 1;
+    e1 = it.ns + max(0, last1 / kChunk - it.c_lo + 1);
+  }
+  const int total = max(e0, e1);
+  it.i0 = (int)((int64_t)total * split / p.splits);
+  const int i1 = (int)((int64_t)total * (split + 1) / p.splits);
+  it.n_it[0] = max(0, min(i1, e0) - it.i0);
+  it.n_it[1] = max(0, min(i1, e1) - it.i0);
+  return it;
+}
+
+// Item of round r for this block; -1: none, and `more` says whether a later
+// round may have one.
+__device__ __forceinline__ int item_index(const Params& p, int r, bool* more) {
+  const int64_t base = (int64_t)r * gridDim.x;
+  *more = base < p.items;
+  const int64_t i = base + ((r & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+  return i < p.items ? (int)i : -1;
+}
+
+// Visible keys [32 w, 32 w + 32) of chunk c for a row at position pos, as bits.
+__device__ __forceinline__ uint32_t mask_word(int base, int pos, int lo, int sinks) {
+  const int hi = pos - base, lw = lo - base, sb = sinks - base;
+  const uint32_t below = hi < 0 ? 0u : (hi >= 31 ? 0xffffffffu : (2u << hi) - 1u);
+  const uint32_t above = lw <= 0 ? 0xffffffffu : (lw >= 32 ? 0u : ~((1u << lw) - 1u));
+  const uint32_t sink = sb <= 0 ? 0u : (sb >= 32 ? 0xffffffffu : (1u << sb) - 1u);
+  return below & (above | sink);
+}
+
+// Pool rows of tokens tok0 + lane + 32 i (-1: not used, or a page id outside
+// the pool, recorded): see attn::token_rows.
+__device__ __forceinline__ void token_rows(const Params& p, const Item& it, int tok0, int lane, int (&rows)[4]) {
+  const int32_t* table = p.page_table + (int64_t)it.b * p.table_stride;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tok = tok0 + lane + 32 * i;
+    rows[i] = -1;
+    if (it.used(p, tok)) {
+      const int64_t pg = resolve_page(__ldg(table + tok), p.num_pages);
+      if (pg >= 0) rows[i] = (int)(((pg * p.B + it.b) * p.Hkv + it.kvh) * p.ps + tok % p.ps);
+      else record_error(MTP_ERR_DEVICE);
+    }
+  }
+}
+
+// Starts the copies of 128 rows into one K or V buffer (layout as TMA's
+// 128-byte swizzle leaves it); rows of -1 and dimensions past D are zero-filled.
+template <int DP>
+__device__ __forceinline__ void fill_tokens(uint8_t* dst, const uint8_t* pool, const int (&rows)[4], int lane, int D) {
+  constexpr int kPieces = DP / 8, kPerCopy = 32 / kPieces;
+  const int j = lane % kPieces, half = j >> 3, jj = j & 7, sub = lane / kPieces;
+  const uint32_t base = smem_u32(dst) + half * kHalfBytes;
+  const bool in = j * 8 < D;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+#pragma unroll
+    for (int u = 0; u < 32 / kPerCopy; ++u) {
+      const int i = 32 * q + kPerCopy * u + sub;
+      const int row = __shfl_sync(0xffffffffu, rows[q], i & 31);
+      const bool go = row >= 0 && in;
+      const uint8_t* src = go ? pool + (int64_t)row * (D * 2) + j * 16 : pool;
+      attn::cp_async16(base + i * 128 + ((jj ^ (i & 7)) << 4), src, go ? 16u : 0u);
+    }
+  }
+}
+
+// AB_FMT: 1 = bf16, 0 = f16; DP: 64 or 128, the head size of the tiles (64 <=
+// D <= DP; the dimensions past D arrive as zeros)
+template <int AB_FMT, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                               const __grid_constant__ CUtensorMap tmV, Params p) {
+  constexpr int kTileBytes = tile_bytes(DP), kNumBuf = num_buf(DP), kHalves = DP / 64;
+  constexpr uint32_t IDESC_S = make_idesc(AB_FMT, 128, kChunk);        // Q (K-major) x K (K-major)
+  constexpr uint32_t IDESC_PV = make_idesc(AB_FMT, 128, DP, 0u, 1u);  // P (K-major) x V (MN-major)
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sBuf = sQ + 2 * kTileBytes;
+  int* sIds = reinterpret_cast<int*>(sBuf + kNumBuf * kTileBytes);  // [kIdRing][kMaxPagesPerChunk]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sIds + kIdRing * kMaxPagesPerChunk);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* buf_full = bars + 2;
+  uint64_t* buf_empty = buf_full + kNumBuf;
+  uint64_t* s_full = buf_empty + kNumBuf;  // [2]
+  uint64_t* p_full = s_full + 2;           // [2 tiles][2 halves of 64 keys]
+  uint64_t* pv_done = p_full + 4;          // [2]
+  uint64_t* ids_full = pv_done + 2;        // [kIdRing]
+  uint64_t* ids_empty = ids_full + kIdRing;
+  uint64_t* drain = ids_empty + kIdRing;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 + 2 * kNumBuf + 2 + 4 + 2 + 2 * kIdRing + 1) * 8 + 8 <= 512, "barrier area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < kNumBuf; ++i) {
+      mbar_init(&buf_full[i], 1);
+      mbar_init(&buf_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[2 * t], 4);  // one arrival per softmax warp
+      mbar_init(&p_full[2 * t + 1], 4);
+      mbar_init(&pv_done[t], 1);
+    }
+    for (int i = 0; i < kIdRing; ++i) {
+      mbar_init(&ids_full[i], 1);
+      mbar_init(&ids_empty[i], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int ppc = p.slab > 0 ? kChunk / p.slab : 0;  // page slabs per chunk
+
+  if (warp >= 8) {  // warpgroup 2: producer, MMA, page table, idle
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsAux));
+    bool ok = true, more = true;
+    if (warp == kWarpProducer) {
+      // -------------------------------------------------------------- producer (whole warp)
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+      }
+      int buffer = 0, chunks = 0, queries = 0;  // buffers, chunks and Q loads so far
+      for (int r = 0; ok; ++r) {
+        const int index = item_index(p, r, &more);
+        if (!more) break;
+        if (index < 0) continue;
+        const Item it = item_of(p, index);
+        const int n_it = it.count();
+        if (n_it == 0) continue;
+        {
+          bool got = true;
+          if (lane == 0) {
+            got = mbar_wait(q_empty, (queries & 1) ^ 1u, abort_flag);
+            if (got) {
+              const int tiles = it.s0 + p.tpt < it.n ? 2 : 1;
+              mbar_expect_tx(q_full, tiles * kHalves * p.tpt * p.G * 128);
+              for (int t = 0; t < tiles; ++t)
+                for (int h = 0; h < kHalves; ++h)
+                  tma_load_4d(sQ + t * kTileBytes + h * kHalfBytes, &tmQ, h * 64, it.kvh * p.G, it.s0 + t * p.tpt,
+                              it.b, q_full);
+            }
+          }
+          ++queries;
+          if (!__shfl_sync(0xffffffffu, got, 0)) break;
+        }
+        for (int i = 0; i < n_it && ok; ++i, ++chunks) {
+          const int c = it.chunk(i);
+          const int slot = chunks % kIdRing;
+          int pg = 0;
+          bool got = true;
+          if (lane == 0) got = mbar_wait(&ids_full[slot], (chunks / kIdRing) & 1, abort_flag);
+          if (!__shfl_sync(0xffffffffu, got, 0)) {
+            ok = false;
+            break;
+          }
+          if (lane < ppc) pg = sIds[slot * kMaxPagesPerChunk + lane];
+          const bool per_token = sIds[slot * kMaxPagesPerChunk] < 0;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ids_empty[slot]);
+          int rows[4];
+          if (per_token) token_rows(p, it, c * kChunk, lane, rows);
+          for (int kv = 0; kv < 2; ++kv, ++buffer) {
+            const int buf = buffer % kNumBuf;
+            got = true;
+            if (lane == 0) {
+              got = mbar_wait(&buf_empty[buf], ((buffer / kNumBuf) & 1) ^ 1u, abort_flag);
+              if (got && !per_token) mbar_expect_tx(&buf_full[buf], kTileBytes);
+            }
+            if (!__shfl_sync(0xffffffffu, got, 0)) {
+              ok = false;
+              break;
+            }
+            __syncwarp();
+            uint8_t* dst = sBuf + buf * kTileBytes;
+            if (per_token) {
+              fill_tokens<DP>(dst, kv ? p.v_pool : p.k_pool, rows, lane, p.D);
+              if (kv == 1) {  // each lane waits for its copies, fences them for the tensor cores, hands both over
+                attn::cp_async_wait_all();
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  mbar_arrive(&buf_full[(buffer - 1) % kNumBuf]);
+                  mbar_arrive(&buf_full[buf]);
+                }
+              }
+            } else if (lane < ppc) {
+              const CUtensorMap* map = kv ? &tmV : &tmK;
+              const int row = ((pg * p.B + it.b) * p.Hkv + it.kvh) * p.ps + (c * kChunk + lane * p.slab) % p.ps;
+#pragma unroll
+              for (int h = 0; h < kHalves; ++h)
+                tma_load_2d(dst + h * kHalfBytes + lane * p.slab * 128, map, h * 64, row, &buf_full[buf]);
+            }
+          }
+        }
+      }
+      attn::cp_async_wait_all();  // after an abort too: no copy of this warp may land after the block's end
+    } else if (warp == kWarpTable) {
+      // -------------------------------------------------------------- page-table warp
+      // Lane l looks at tokens 4 l .. 4 l + 3 of a chunk: page-granular if all
+      // tokens of every slab lie in the page of the slab's first one.
+      int chunks = 0;
+      for (int r = 0; ok; ++r) {
+        const int index = item_index(p, r, &more);
+        if (!more) break;
+        if (index < 0) continue;
+        const Item it = item_of(p, index);
+        const int n_it = it.count();
+        const int32_t* table = p.page_table + (int64_t)it.b * p.table_stride;
+        for (int i = 0; i < n_it; ++i, ++chunks) {
+          const int c = it.chunk(i);
+          const int slot = chunks % kIdRing;
+          int id[4] = {-1, -1, -1, -1};
+          const bool whole = p.slab > 0 && it.whole(p, c);  // then all 128 columns are inside the table
+          if (whole) {
+            const int32_t* src = table + c * kChunk + lane * 4;
+            if (p.table_vec) {
+              const int4 e = __ldg(reinterpret_cast<const int4*>(src));
+              id[0] = e.x, id[1] = e.y, id[2] = e.z, id[3] = e.w;
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) id[k] = __ldg(src + k);
+            }
+          }
+          bool got = true;
+          if (lane == 0) got = mbar_wait(&ids_empty[slot], ((chunks / kIdRing) & 1) ^ 1u, abort_flag);
+          if (!__shfl_sync(0xffffffffu, got, 0)) {
+            ok = false;
+            break;
+          }
+          const int page = whole ? (int)resolve_page(id[0], p.num_pages) : -1;
+          bool gran = page >= 0;
+#pragma unroll
+          for (int k = 1; k < 4; ++k) gran &= (int)resolve_page(id[k], p.num_pages) == page;
+          const int per_slab = p.slab > 0 ? p.slab / 4 : 1;  // lanes of a slab
+          const int head = __shfl_sync(0xffffffffu, page, lane / per_slab * per_slab);
+          gran = __all_sync(0xffffffffu, gran && head == page);
+          const int mine = __shfl_sync(0xffffffffu, page, (lane * per_slab) & 31);
+          if (lane < max(ppc, 1)) sIds[slot * kMaxPagesPerChunk + lane] = gran ? mine : -1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ids_full[slot]);
+        }
+      }
+    } else if (warp == kWarpMma && lane == 0) {
+      // -------------------------------------------------------------- MMA issuer
+      int buffer = 0, queries = 0;
+      int done[2] = {0, 0};  // chunks of each tile so far
+      auto wait_buffer = [&](int k) -> bool {
+        return mbar_wait(&buf_full[k % kNumBuf], (k / kNumBuf) & 1, abort_flag);
+      };
+      auto issue_s = [&](int t, int k) {
+        const uint32_t d = tmem_base + (uint32_t)(t * 128);
+        const uint32_t qa = smem_u32(sQ + t * kTileBytes), ka = smem_u32(sBuf + (k % kNumBuf) * kTileBytes);
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+          const uint32_t off = (x >> 2) * kHalfBytes + (x & 3) * 32;
+          umma_f16(d, sw128_kmajor_desc(qa + off), sw128_kmajor_desc(ka + off), IDESC_S, x > 0);
+        }
+        umma_commit(&s_full[t]);
+      };
+      // O_t += P_t V for keys [64 * half, 64 * half + 64) of the chunk
+      auto issue_pv = [&](int t, int k, int half, bool acc) {
+        const uint32_t d = tmem_base + (uint32_t)(256 + t * 128);
+        const uint32_t pa = tmem_base + (uint32_t)(t * 128);
+        const uint32_t va = smem_u32(sBuf + (k % kNumBuf) * kTileBytes);
+#pragma unroll
+        for (int x = 4 * half; x < 4 * half + 4; ++x)
+          umma_f16_ts(d, pa + x * 8, sw128_mnmajor_desc(va + x * 16 * 128, kHalfBytes), IDESC_PV,
+                      (acc || x > 0) ? 1u : 0u);
+      };
+      for (int r = 0; ok; ++r) {
+        const int index = item_index(p, r, &more);
+        if (!more) break;
+        if (index < 0) continue;
+        const Item it = item_of(p, index);
+        const int n_it = it.count();
+        if (n_it == 0) continue;
+        if (!(ok = mbar_wait(q_full, queries & 1, abort_flag))) break;
+        ++queries;
+        if (!(ok = wait_buffer(buffer))) break;
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t)
+          if (it.n_it[t] > 0) issue_s(t, buffer);
+        umma_commit(&buf_empty[buffer % kNumBuf]);
+        if (n_it == 1) umma_commit(q_empty);
+        for (int i = 0; i < n_it && ok; ++i, buffer += 2) {
+          const int v = buffer + 1, knext = buffer + 2;
+          const int t_first = i < it.n_it[0] ? 0 : 1;                                  // tiles that take chunk i
+          const int t_last = i < it.n_it[1] ? 1 : 0;
+          const int s_first = i + 1 < it.n_it[0] ? 0 : 1, s_last = i + 1 < it.n_it[1] ? 1 : 0;  // and chunk i + 1
+          for (int t = t_first; t <= t_last && ok; ++t) {
+            if (!(ok = mbar_wait(&p_full[2 * t], done[t] & 1, abort_flag))) break;
+            tc_fence_after();
+            if (t == t_first) {
+              if (!(ok = wait_buffer(v))) break;
+              tc_fence_after();
+            }
+            issue_pv(t, v, 0, i > 0);
+            if (!(ok = mbar_wait(&p_full[2 * t + 1], done[t] & 1, abort_flag))) break;
+            tc_fence_after();
+            issue_pv(t, v, 1, true);
+            umma_commit(&pv_done[t]);
+            ++done[t];
+            if (t == t_last) umma_commit(&buf_empty[v % kNumBuf]);
+            if (i + 1 < it.n_it[t]) {
+              if (t == s_first) {
+                if (!(ok = wait_buffer(knext))) break;
+                tc_fence_after();
+              }
+              issue_s(t, knext);
+              if (t == s_last) {
+                umma_commit(&buf_empty[knext % kNumBuf]);
+                if (i + 2 == n_it) umma_commit(q_empty);
+              }
+            }
+          }
+        }
+      }
+      umma_commit(drain);
+      mbar_wait(drain, 0, abort_flag, /*honour_abort=*/false);
+    }
+  } else {  // warpgroups 0-1: softmax of query tiles 0 and 1
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int t = warp / 4;
+    const int q = warp & 3;
+    const int row = q * 32 + lane;  // row within the tile == TMEM lane
+    const int row_s = row / p.G, g = row % p.G;
+    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_off + (uint32_t)(t * 128);
+    const uint32_t o_addr = tmem_base + lane_off + (uint32_t)(256 + t * 128);
+    int done = 0;  // chunks of this tile so far
+    bool ok = true, more = true;
+    for (int r = 0; ok; ++r) {
+      const int index = item_index(p, r, &more);
+      if (!more) break;
+      if (index < 0) continue;
+      const Item it = item_of(p, index);
+      const int s = it.s0 + t * p.tpt + row_s;  // row of the call
+      const bool in_tile = row_s < p.tpt && s < p.S;
+      const bool row_ok = in_tile && s < it.n;
+      const int pos = row_ok ? it.len - it.n + s : -1;
+      const int lo = pos - p.window + 1;
+      const int n_it = it.n_it[t];
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int i = 0; i < n_it; ++i) {
+        const int first = it.chunk(i) * kChunk;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (done + i) & 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const bool no_masked = first + kChunk - 1 <= pos && (first >= lo || first + kChunk <= p.sinks);
+        uint32_t sc[128];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tmem_ld32(s_addr + j * 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[32 * j]));
+        tmem_wait_ld();
+        if (!no_masked) {
+          uint32_t mw[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) mw[w] = mask_word(first + 32 * w, pos, lo, p.sinks);
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if (!((mw[j >> 5] >> (j & 31)) & 1u)) sc[j] = 0xff800000u;  // -inf
+        }
+        float m8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(sc[k]), __uint_as_float(sc[k + 8]));
+#pragma unroll
+        for (int j = 16; j < 128; j += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            m8[k] = attn::fmax3(m8[k], __uint_as_float(sc[j + k]), __uint_as_float(sc[j + 8 + k]));
+        const float mx = p.scale_log2 * attn::fmax3(attn::fmax3(m8[0], m8[1], m8[2]),
+                                                    attn::fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+        const float m_new = fmaxf(m_run, mx);
+        if (i > 0) {
+          // P and O may be touched only after the previous PV completed
+          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], (done + i - 1) & 1, abort_flag))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const bool need = m_new > m_run + attn::kRescaleThreshold;
+          if (__any_sync(0xffffffffu, need)) {
+            const float alpha = need ? attn::ex2(m_run - m_new) : 1.0f;
+#pragma unroll 1
+            for (int j = 0; j < DP / 16; ++j) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + j * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st16(o_addr + j * 16, o);
+            }
+            tmem_wait_st();
+            if (need) {
+              l_run *= alpha;
+              m_run = m_new;
+            }
+          }
+        } else {
+          m_run = m_new;
+        }
+        const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+        float ls0 = 0.f, ls1 = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          attn::exp_pack_half<AB_FMT>(sc, h, p.scale_log2, m_use, ls0, ls1);
+          tmem_st32(s_addr + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(&sc[32 * h]));
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
+        }
+        l_run += ls0 + ls1;
+      }
+      if (!ok) break;
+      done += n_it;
+      if (n_it > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[t], (done - 1) & 1, abort_flag))) break;
+      tc_fence_after();
+      if (p.splits == 1) {
+        const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+        uint8_t* orow = static_cast<uint8_t*>(p.out) +
+                        ((((int64_t)it.b * p.S + s) * p.Hq + (int64_t)it.kvh * p.G + g) * p.D) * 2;
+#pragma unroll 1
+        for (int j = 0; j < DP / 32; ++j) {
+          uint32_t o[32];
+          if (n_it > 0) {
+            tmem_ld32(o_addr + j * 32, o);
+            tmem_wait_ld();
+          }
+          if (in_tile) {
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              w[k] = row_ok ? attn::pack_bf16(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv,
+                                              AB_FMT == 1 ? MTP_DTYPE_BF16 : MTP_DTYPE_F16)
+                            : 0u;  // rows behind q_lens
+            uint4* dst = reinterpret_cast<uint4*>(orow + j * 64);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (j * 32 + k * 8 < p.D) dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+          }
+        }
+      } else if (n_it > 0 || row_ok) {
+        const int64_t slot = (int64_t)index * 256 + t * 128 + row;
+        float* po = p.part_o + slot * p.D;
+#pragma unroll 1
+        for (int j = 0; j < (n_it > 0 ? DP / 32 : 0); ++j) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + j * 32, o);
+          tmem_wait_ld();
+          if (row_ok) {
+            float4* dst = reinterpret_cast<float4*>(po + j * 32);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (j * 32 + k * 4 < p.D)
+                dst[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                     __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+          }
+        }
+        if (row_ok) {
+          p.part_ml[slot * 2] = m_run;  // -inf: no key of this piece is visible, and its output is not read
+          p.part_ml[slot * 2 + 1] = l_run;
+        }
+      }
+      // the next item's products overwrite O only after this warp's next arrival at p_full
+      tc_fence_before();
+      __syncwarp();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Joins the pieces of each row (splits > 1), in their order; zero for rows
+// behind q_lens.  One warp per row of the call.
+template <typename T>
+__global__ void __launch_bounds__(256) prompt_merge_kernel(Params p) {
+  const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (row >= (int64_t)p.B * p.S * p.Hq) return;
+  const int h = (int)(row % p.Hq), s = (int)(row / p.Hq % p.S), b = (int)(row / p.Hq / p.S);
+  const int kvh = h / p.G, g = h % p.G;
+  const int pair = s / (2 * p.tpt), t = s / p.tpt % 2, r = (s % p.tpt) * p.G + g;
+  const int64_t base = (((int64_t)(p.pairs - 1 - pair) * p.B + b) * p.Hkv + kvh) * p.splits;
+  const int cap = (int)min(p.table_stride, (int64_t)INT32_MAX);
+  const int len = max(0, min(p.seq_lens[b], cap));
+  const int n = max(0, min(p.q_lens ? p.q_lens[b] : p.S, min(p.S, len)));
+  T* out = static_cast<T*>(p.out) + row * p.D;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
+  const bool mine = lane * 4 < p.D;
+  if (s < n) {
+    float M = -INFINITY;
+    for (int i = 0; i < p.splits; ++i) M = fmaxf(M, p.part_ml[((base + i) * 256 + t * 128 + r) * 2]);
+#pragma unroll 4
+    for (int i = 0; i < p.splits; ++i) {
+      const int64_t slot = (base + i) * 256 + t * 128 + r;
+      const float m = p.part_ml[slot * 2];
+      if (m == -INFINITY) continue;
+      const float w = attn::ex2(m - M);
+      L += w * p.part_ml[slot * 2 + 1];
+      if (mine) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot * p.D + lane * 4);
+        acc[0] += w * v.x;
+        acc[1] += w * v.y;
+        acc[2] += w * v.z;
+        acc[3] += w * v.w;
+      }
+    }
+  }
+  const float inv = L > 0.f ? 1.0f / L : 0.f;
+  if (mine)
+    *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(split::Mma<T>::pack(acc[0] * inv, acc[1] * inv),
+                                                           split::Mma<T>::pack(acc[2] * inv, acc[3] * inv));
+}
+
+}  // namespace prompt
+}  // namespace mtp

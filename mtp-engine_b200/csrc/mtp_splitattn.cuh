@@ -54,7 +54,7 @@ struct Args {
   const int32_t* seq_lens;  // [B]
   const int32_t* q_lens;    // [B]; null: S each (decode: the one token of every non-empty sequence)
   int B, S, Hq, Hkv, G, D, dtype;
-  int window;  // INT_MAX: everything
+  int window;  // 2^30: everything
   int sinks;
   float scale, scale_log2;
   int row_tiles;    // ceil(S * G / kRows)
