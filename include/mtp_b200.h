@@ -311,6 +311,10 @@ int mtp_paged_kv_write(void* k_pages, void* v_pages, int dtype, const int32_t* p
 /* serving from a paged cache (no counterparts in the reference)              */
 /* ------------------------------------------------------------------------- */
 
+/* These entries take their arguments in a struct whose members are 8 bytes
+ * each (pointers, int64_t, double): a host that calls them once per layer and
+ * token fills it in one go. */
+
 /* RMSNorm of every query and key head and the position rotation, in one pass;
  * with a page table also the write of the keys and values into the pool.
  * Per head x of D values:
@@ -332,14 +336,36 @@ int mtp_paged_kv_write(void* k_pages, void* v_pages, int dtype, const int32_t* p
  * position outside the tables, or a page id outside the pool, is recorded
  * (MTP_ERR_DEVICE) and that token is not written (its query row is zero when
  * its position has no angle). */
-int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const void* k, int64_t k_sb,
-                     int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
-                     const int32_t* positions, const float* cos, const float* sin, int64_t max_pos, int64_t rot_dim,
-                     const void* q_weight, int q_weight_dtype, const void* k_weight, int k_weight_dtype, float eps,
-                     int normalise, int interleaved, void* q_out, void* k_out, void* k_pages, void* v_pages,
-                     const int32_t* page_table, int64_t table_stride, int64_t num_pages, int64_t page_size,
-                     const int32_t* start, const int32_t* count, int64_t B, int64_t S, int64_t Hq, int64_t Hkv,
-                     int64_t D, void* stream);
+typedef struct {
+  const void* q;
+  int64_t q_stride[3]; /* elements: sequence, token, head */
+  const void* k;
+  int64_t k_stride[3];
+  const void* v;
+  int64_t v_stride[3];
+  int64_t dtype;
+  const int32_t* positions;
+  const float* cos;
+  const float* sin;
+  int64_t max_pos, rot_dim;
+  const void* q_weight;
+  int64_t q_weight_dtype;
+  const void* k_weight;
+  int64_t k_weight_dtype;
+  double eps;
+  int64_t normalise, interleaved;
+  void* q_out;
+  void* k_out;
+  void* k_pages;
+  void* v_pages;
+  const int32_t* page_table;
+  int64_t table_stride, num_pages, page_size;
+  const int32_t* start;
+  const int32_t* count;
+  int64_t B, S, Hq, Hkv, D;
+  void* stream;
+} mtp_qk_norm_rope_args;
+int mtp_qk_norm_rope(const mtp_qk_norm_rope_args* args);
 
 /* Bytes of workspace mtp_paged_window_attention needs; max_keys is the page
  * table's width.  The workspace holds nothing between calls. */
@@ -362,12 +388,25 @@ size_t mtp_paged_window_attention_workspace(int64_t B, int64_t S, int64_t Hq, in
  * recorded (MTP_ERR_DEVICE).
  * key_weights (S == 1; may be NULL) [B,Hkv,weight_ld] float32: every visible
  * key's softmax weight, summed over the heads that share it, is added. */
-int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
-                               int64_t table_stride, const int32_t* seq_lens, const int32_t* q_lens, void* out,
-                               int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
-                               int64_t num_pages, int64_t page_size, float scale, int64_t window, int64_t sinks,
-                               float* key_weights, int64_t weight_ld, void* workspace, size_t workspace_bytes,
-                               void* stream);
+typedef struct {
+  const void* q;
+  const void* k_pages;
+  const void* v_pages;
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;
+  void* out;
+  int64_t dtype, B, S, Hq, Hkv, D, num_pages, page_size;
+  double scale;
+  int64_t window, sinks;
+  float* key_weights;
+  int64_t weight_ld;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} mtp_paged_window_attention_args;
+int mtp_paged_window_attention(const mtp_paged_window_attention_args* args);
 
 /* Bytes of workspace mtp_paged_kv_evict needs (it holds nothing between calls). */
 size_t mtp_paged_kv_evict_workspace(int64_t B, int64_t H, int64_t budget);
@@ -382,11 +421,23 @@ size_t mtp_paged_kv_evict_workspace(int64_t B, int64_t H, int64_t budget);
  * Shorter sequences stay as they are.  The positions of a sequence own a slot
  * each: with a table that maps two of them to one slot the rows moved there
  * are unspecified.  Pools f32, bf16 or f16. */
-int mtp_paged_kv_evict(void* k_pages, void* v_pages, int dtype, const int32_t* page_table, int64_t table_stride,
-                       int64_t num_pages, int64_t page_size, const int32_t* seq_lens, float* key_weights,
-                       int64_t weight_ld, int32_t* kept, int32_t* new_lens, int64_t B, int64_t H, int64_t D,
-                       int64_t budget, int64_t sinks, int64_t recent, void* workspace, size_t workspace_bytes,
-                       void* stream);
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  int64_t dtype;
+  const int32_t* page_table;
+  int64_t table_stride, num_pages, page_size;
+  const int32_t* seq_lens;
+  float* key_weights;
+  int64_t weight_ld;
+  int32_t* kept;
+  int32_t* new_lens;
+  int64_t B, H, D, budget, sinks, recent;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} mtp_paged_kv_evict_args;
+int mtp_paged_kv_evict(const mtp_paged_kv_evict_args* args);
 
 /* ------------------------------------------------------------------------- */
 /* verification (lm_head GEMM -> argmax -> acceptance)                        */

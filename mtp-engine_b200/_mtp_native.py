@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -53,15 +54,11 @@ SIGNATURES = {
                                           _i64, _i64, _i64, _f, _f, _vp, _sz, _vp]),
     "mtp_paged_kv_write": (_i, [_vp, _vp, _i, _vp, _i64, _i64, _i64, _vp, _vp, _i, _i64, _vp, _vp, _i64, _i64,
                                 _i64, _i64, _i64, _vp]),
-    "mtp_qk_norm_rope": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i, _vp, _vp,
-                              _vp, _i64, _i64, _vp, _i, _vp, _i, _f, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
-                              _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "mtp_qk_norm_rope": (_i, [ctypes.c_char_p]),
     "mtp_paged_window_attention_workspace": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i]),
-    "mtp_paged_window_attention": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64,
-                                        _i64, _i64, _f, _i64, _i64, _vp, _i64, _vp, _sz, _vp]),
+    "mtp_paged_window_attention": (_i, [ctypes.c_char_p]),
     "mtp_paged_kv_evict_workspace": (_sz, [_i64, _i64, _i64]),
-    "mtp_paged_kv_evict": (_i, [_vp, _vp, _i, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64,
-                                _i64, _i64, _i64, _vp, _sz, _vp]),
+    "mtp_paged_kv_evict": (_i, [ctypes.c_char_p]),
     "mtp_verify_workspace": (_sz, [_i64]),
     "mtp_verify_workspace_init": (_i, [_vp, _sz, _vp]),
     "mtp_fused_verify": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
@@ -104,6 +101,13 @@ SIGNATURES = {
     "mtp_fused_multi_verify_noalloc": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                             _i64, _vp]),
 }
+
+# argument structs of include/mtp_b200.h (8-byte members, pointers as integers,
+# 0 for NULL), filled in one go: a ctypes call with 40 arguments costs more
+# than the smallest kernels behind it
+QK_NORM_ROPE_ARGS = struct.Struct("=12q q 3q 2q 4q d 2q 4q 4q 2q 5q q")
+WINDOW_ATTENTION_ARGS = struct.Struct("=4q q 3q 8q d 2q 2q 2q q")
+KV_EVICT_ARGS = struct.Struct("=2q 2q 3q 2q q 2q 6q 2q q")
 
 _lib = None
 _lib_lock = threading.Lock()
@@ -181,14 +185,38 @@ def stream_handle(device: torch.device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call_on(device: torch.device, fn, *args) -> int:
-    """fn(*args) with `device` current (the library launches on the current
-    device; the stream among the arguments belongs to `device`)."""
-    idx = device.index
-    if idx is None or idx == torch.cuda.current_device():
+def same_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
+    """Index of the CUDA device that holds all of the tensors (None: skipped);
+    raises as require_cuda does."""
+    idx = first.get_device()
+    if idx < 0:
+        require_cuda(first)
+    for t in rest:
+        if t is not None and t.get_device() != idx:
+            require_cuda(first, t)
+    return idx
+
+
+def address(t: Optional[torch.Tensor]) -> int:
+    """Device address of t for an argument struct (0 for NULL)."""
+    return 0 if t is None else t.data_ptr()
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def call_on(idx: int, fn, *args) -> int:
+    """fn(*args) with device `idx` current (the library launches on the current
+    device; a stream among the arguments belongs to `idx`)."""
+    if idx == _current_device():
         return fn(*args)
     with torch.cuda.device(idx):
         return fn(*args)
+
+
+def stream_of(idx: int) -> int:
+    """The current torch stream of device `idx` as a cudaStream_t value."""
+    return _raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream
 
 
 # --------------------------------------------------------------------------- #

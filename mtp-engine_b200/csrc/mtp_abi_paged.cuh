@@ -29,10 +29,12 @@ int launch_dependent(Kern kern, unsigned grid_x, unsigned grid_y, int threads, c
   return MTP_OK;
 }
 
+// a dtype code from an 8-byte member, out of range where it is none
+int code(int64_t dtype) { return dtype >= 0 && dtype <= MTP_DTYPE_E4M3 ? (int)dtype : -1; }
+
 bool pool_fits(int64_t P, int64_t B, int64_t H, int64_t ps) {
   // rows of the pool are numbered in 32 bits (a row is D elements)
-  const double rows = (double)P * B * H * ps;
-  return rows < 2147483647.0;
+  return (double)P * B * H * ps < 2147483647.0;
 }
 
 // ---------------------------------------------------------------- norm + rotation
@@ -249,15 +251,17 @@ int launch_move(const evict::Args& a, int words, int lanes, cudaStream_t s) {
 
 extern "C" {
 
-int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const void* k, int64_t k_sb,
-                     int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
-                     const int32_t* positions, const float* cos, const float* sin, int64_t max_pos, int64_t rot_dim,
-                     const void* q_weight, int q_weight_dtype, const void* k_weight, int k_weight_dtype, float eps,
-                     int normalise, int interleaved, void* q_out, void* k_out, void* k_pages, void* v_pages,
-                     const int32_t* page_table, int64_t table_stride, int64_t num_pages, int64_t page_size,
-                     const int32_t* start, const int32_t* count, int64_t B, int64_t S, int64_t Hq, int64_t Hkv,
-                     int64_t D, void* stream) {
+int mtp_qk_norm_rope(const mtp_qk_norm_rope_args* args) {
   MTP_NVTX("mtp_qk_norm_rope");
+  if (!args) return fail(MTP_ERR_ARG, "null arguments");
+  const mtp_qk_norm_rope_args& g = *args;
+  const int64_t B = g.B, S = g.S, Hq = g.Hq, Hkv = g.Hkv, D = g.D, rot_dim = g.rot_dim, max_pos = g.max_pos;
+  const int64_t table_stride = g.table_stride, num_pages = g.num_pages, page_size = g.page_size;
+  const int dtype = code(g.dtype), q_weight_dtype = code(g.q_weight_dtype), k_weight_dtype = code(g.k_weight_dtype);
+  const void *q = g.q, *k = g.k, *v = g.v, *q_weight = g.q_weight, *k_weight = g.k_weight;
+  void *q_out = g.q_out, *k_out = g.k_out, *k_pages = g.k_pages, *v_pages = g.v_pages;
+  const int32_t *positions = g.positions, *page_table = g.page_table, *start = g.start;
+  const float *cos = g.cos, *sin = g.sin;
   const bool paged = page_table != nullptr;
   if (B < 0 || S < 0 || Hq < 0 || Hkv < 0 || D <= 0 || max_pos < 0 || rot_dim < 0)
     return fail(MTP_ERR_SHAPE, "bad norm/rotation sizes");
@@ -280,7 +284,7 @@ int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, co
     return fail(MTP_ERR_SHAPE, "too many rows");
   rope::Args a{};
   const void* x[3] = {q, k, v};
-  const int64_t st[3][3] = {{q_sb, q_ss, q_sh}, {k_sb, k_ss, k_sh}, {v_sb, v_ss, v_sh}};
+  const int64_t* st[3] = {g.q_stride, g.k_stride, g.v_stride};
   for (int i = 0; i < 3; ++i) {
     a.x[i] = x[i];
     a.sb[i] = st[i][0];
@@ -296,9 +300,9 @@ int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, co
   a.w[1] = k_weight;
   a.w_dtype[0] = q_weight_dtype;
   a.w_dtype[1] = k_weight_dtype;
-  a.eps = eps;
-  a.normalise = normalise;
-  a.interleaved = interleaved;
+  a.eps = (float)g.eps;
+  a.normalise = g.normalise != 0;
+  a.interleaved = g.interleaved != 0;
   a.q_out = q_out;
   a.k_out = paged ? nullptr : k_out;
   a.pages[0] = k_pages;
@@ -308,7 +312,7 @@ int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, co
   a.num_pages = num_pages;
   a.page_size = page_size;
   a.start = paged ? start : nullptr;
-  a.count = count;
+  a.count = g.count;
   a.B = (int)B;
   a.S = (int)S;
   a.Hq = (int)Hq;
@@ -316,7 +320,7 @@ int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, co
   a.D = (int)D;
   a.dtype = dtype;
   const int e16 = 16 / dtype_bytes(dtype);  // elements in 16 bytes
-  bool vec = D % 8 == 0 && D <= 256 && (interleaved ? a.half % 4 == 0 : a.half % 8 == 0) && aligned16(cos) &&
+  bool vec = D % 8 == 0 && D <= 256 && (a.interleaved ? a.half % 4 == 0 : a.half % 8 == 0) && aligned16(cos) &&
              aligned16(sin) && aligned16(q_out) && aligned16(a.k_out);
   for (int i = 0; i < (paged ? 3 : 2); ++i) {
     vec &= aligned16(x[i]);
@@ -325,7 +329,7 @@ int mtp_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, co
   if (paged) vec &= aligned16(k_pages) && aligned16(v_pages);
   int dev;
   if (int r = current_device(&dev)) return r;
-  const cudaStream_t s = as_stream(stream);
+  const cudaStream_t s = as_stream(g.stream);
   if (!vec) {
     const int64_t rows = B * S * heads, blocks = (rows + rope::kThreads / 32 - 1) / (rope::kThreads / 32);
     if (blocks > INT32_MAX) return fail(MTP_ERR_SHAPE, "too many rows");
@@ -354,13 +358,20 @@ size_t mtp_paged_window_attention_workspace(int64_t B, int64_t S, int64_t Hq, in
   return window_plan(B, S, Hq, Hkv, D, max_keys, window, sinks, dtype, true, with_weights != 0).total();
 }
 
-int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
-                               int64_t table_stride, const int32_t* seq_lens, const int32_t* q_lens, void* out,
-                               int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
-                               int64_t num_pages, int64_t page_size, float scale, int64_t window, int64_t sinks,
-                               float* key_weights, int64_t weight_ld, void* workspace, size_t workspace_bytes,
-                               void* stream) {
+int mtp_paged_window_attention(const mtp_paged_window_attention_args* args) {
   MTP_NVTX("mtp_paged_window_attention");
+  if (!args) return fail(MTP_ERR_ARG, "null arguments");
+  const mtp_paged_window_attention_args& g = *args;
+  const int64_t B = g.B, S = g.S, Hq = g.Hq, Hkv = g.Hkv, D = g.D, num_pages = g.num_pages, page_size = g.page_size;
+  const int64_t table_stride = g.table_stride, window = g.window, sinks = g.sinks, weight_ld = g.weight_ld;
+  const int dtype = code(g.dtype);
+  const void *q = g.q, *k_pages = g.k_pages, *v_pages = g.v_pages;
+  void *out = g.out, *workspace = g.workspace;
+  const int32_t *page_table = g.page_table, *seq_lens = g.seq_lens, *q_lens = g.q_lens;
+  float* key_weights = g.key_weights;
+  const float scale = (float)g.scale;
+  const size_t workspace_bytes = g.workspace_bytes > 0 ? (size_t)g.workspace_bytes : 0;
+  const cudaStream_t s = as_stream(g.stream);
   if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || page_size <= 0 || num_pages < 0 || table_stride < 0 ||
       window < 0 || sinks < 0)
     return fail(MTP_ERR_SHAPE, "bad window attention sizes");
@@ -382,7 +393,6 @@ int mtp_paged_window_attention(const void* q, const void* k_pages, const void* v
       window_plan(B, S, Hq, Hkv, D, table_stride, window, sinks, dtype, aligned, key_weights != nullptr);
   if (!workspace || workspace_bytes < p.total() || !aligned16(workspace))
     return fail(MTP_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, needed", p.total());
-  const cudaStream_t s = as_stream(stream);
   split::Args a{};
   a.q = q;
   a.out = out;
@@ -440,12 +450,20 @@ size_t mtp_paged_kv_evict_workspace(int64_t B, int64_t H, int64_t budget) {
   return align256((size_t)B * H * budget * 8) + 256;
 }
 
-int mtp_paged_kv_evict(void* k_pages, void* v_pages, int dtype, const int32_t* page_table, int64_t table_stride,
-                       int64_t num_pages, int64_t page_size, const int32_t* seq_lens, float* key_weights,
-                       int64_t weight_ld, int32_t* kept, int32_t* new_lens, int64_t B, int64_t H, int64_t D,
-                       int64_t budget, int64_t sinks, int64_t recent, void* workspace, size_t workspace_bytes,
-                       void* stream) {
+int mtp_paged_kv_evict(const mtp_paged_kv_evict_args* args) {
   MTP_NVTX("mtp_paged_kv_evict");
+  if (!args) return fail(MTP_ERR_ARG, "null arguments");
+  const mtp_paged_kv_evict_args& g = *args;
+  const int64_t B = g.B, H = g.H, D = g.D, budget = g.budget, sinks = g.sinks, recent = g.recent;
+  const int64_t table_stride = g.table_stride, num_pages = g.num_pages, page_size = g.page_size;
+  const int64_t weight_ld = g.weight_ld;
+  const int dtype = code(g.dtype);
+  void *k_pages = g.k_pages, *v_pages = g.v_pages, *workspace = g.workspace;
+  const int32_t *page_table = g.page_table, *seq_lens = g.seq_lens;
+  float* key_weights = g.key_weights;
+  int32_t *kept = g.kept, *new_lens = g.new_lens;
+  const size_t workspace_bytes = g.workspace_bytes > 0 ? (size_t)g.workspace_bytes : 0;
+  const cudaStream_t s = as_stream(g.stream);
   if (B < 0 || H <= 0 || D <= 0 || page_size <= 0 || num_pages < 0 || table_stride < 0 || weight_ld < 0 ||
       budget < 0 || sinks < 0 || recent < 0)
     return fail(MTP_ERR_SHAPE, "bad eviction sizes");
@@ -484,7 +502,6 @@ int mtp_paged_kv_evict(void* k_pages, void* v_pages, int dtype, const int32_t* p
   a.recent = (int)recent;
   int dev;
   if (int st = current_device(&dev)) return st;
-  const cudaStream_t s = as_stream(stream);
   evict::evict_select_kernel<<<(unsigned)(B * H), evict::kThreads, 0, s>>>(a);
   MTP_LAUNCH_CHECK();
   if (budget == 0 || table_stride <= budget || weight_ld <= budget) return MTP_OK;  // no sequence is longer

@@ -40,6 +40,7 @@ the reference's engine keeps working); otherwise they raise AttributeError.
 
 from __future__ import annotations
 
+import functools
 import importlib.util
 import math
 import os
@@ -436,49 +437,60 @@ def _qk_norm_rope(q, k, v, positions, cos, sin, q_weight, k_weight, eps, interle
                   start, count, what):
     q, k = _rows(q), _rows(k)
     B, S, Hq, D = q.shape
-    Hkv = k.shape[2]
-    assert k.shape == (B, S, Hkv, D), f"q is {tuple(q.shape)}, k is {tuple(k.shape)}"
-    assert k.dtype == q.dtype
+    dtype = q.dtype
+    kshape = k.shape
+    Hkv = kshape[2]
+    assert kshape == (B, S, Hkv, D) and k.dtype is dtype, f"q is {tuple(q.shape)}, k is {tuple(kshape)}"
     cos, sin = cos.contiguous(), sin.contiguous()
-    assert cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32, \
+    max_pos, half = cos.shape
+    assert sin.shape == (max_pos, half) and cos.dtype is torch.float32 and sin.dtype is torch.float32, \
         "cos and sin are float32 [positions, rotated / 2]"
     if positions is not None:
         positions = _i32(positions)
         assert positions.shape == (B, S)
-    for w in (q_weight, k_weight):
-        assert w is None or w.shape == (D,), "norm weights must have shape [D]"
     if q_weight is not None:
         q_weight = q_weight.contiguous()
+        assert q_weight.shape == (D,), "norm weights must have shape [D]"
     if k_weight is not None:
         k_weight = k_weight.contiguous()
-    P = ps = width = 0
-    vs = (0, 0, 0)
+        assert k_weight.shape == (D,), "norm weights must have shape [D]"
+    code, ptr = _N.dtype_code, _N.address
+    kv, pages, vs = (0, 0), (0, 0, 0, 0), (0, 0, 0)
+    k_out = None
     if page_table is not None:
         v = _rows(v)
-        assert v.shape == k.shape and v.dtype == q.dtype
+        assert v.shape == kshape and v.dtype is dtype
         assert k_pages.is_contiguous() and v_pages.is_contiguous(), "page pools are written in place"
         P, Bp, Hp, ps, Dp = k_pages.shape
-        assert (Bp, Hp, Dp) == (B, Hkv, D) and v_pages.shape == k_pages.shape
-        assert k_pages.dtype == q.dtype and v_pages.dtype == q.dtype
+        assert Bp == B and Hp == Hkv and Dp == D and v_pages.shape == k_pages.shape
+        assert k_pages.dtype is dtype and v_pages.dtype is dtype
         page_table, start = _i32(page_table), _i32(start)
-        assert page_table.dim() == 2 and page_table.shape[0] == B and start.shape == (B,)
-        width, vs = page_table.shape[1], v.stride()
+        assert page_table.dim() == 2, "page_table is [B, L]"
+        Bt, width = page_table.shape
+        assert Bt == B and start.shape == (B,)
         if count is not None:
             count = _i32(count)
             assert count.shape == (B,)
-    dev = _N.require_cuda(q, k, v if page_table is not None else None, positions, cos, sin, q_weight, k_weight,
-                          k_pages, v_pages, page_table, start, count)
-    q_out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=q.device)
-    k_out = None if page_table is not None else torch.empty((B, Hkv, S, D), dtype=q.dtype, device=q.device)
+        dev = _N.same_device(q, k, v, positions, cos, sin, q_weight, k_weight, k_pages, v_pages, page_table, start,
+                             count)
+        vs = v.stride()
+        kv, pages = (k_pages.data_ptr(), v_pages.data_ptr()), (page_table.data_ptr(), width, P, ps)
+    else:
+        dev = _N.same_device(q, k, positions, cos, sin, q_weight, k_weight)
+        v = None
+        k_out = torch.empty((B, Hkv, S, D), dtype=dtype, device=q.device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     qs, ks = q.stride(), k.stride()
-    ptr, code = _N.ptr, _N.dtype_code
-    _N.check(_N.call_on(
-        dev, _N.lib().mtp_qk_norm_rope, ptr(q), qs[0], qs[1], qs[2], ptr(k), ks[0], ks[1], ks[2],
-        ptr(v) if page_table is not None else None, vs[0], vs[1], vs[2], code(q), ptr(positions), ptr(cos), ptr(sin),
-        cos.shape[0], 2 * cos.shape[1], ptr(q_weight), 0 if q_weight is None else code(q_weight), ptr(k_weight),
-        0 if k_weight is None else code(k_weight), 0.0 if eps is None else float(eps), int(eps is not None),
-        int(interleaved), ptr(q_out), ptr(k_out), ptr(k_pages), ptr(v_pages), ptr(page_table), width, P, ps,
-        ptr(start), ptr(count), B, S, Hq, Hkv, D, _N.stream_handle(dev)), what)
+    args = _N.QK_NORM_ROPE_ARGS.pack(
+        q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], ptr(v), vs[0], vs[1], vs[2], code(q),
+        ptr(positions), cos.data_ptr(), sin.data_ptr(), max_pos, 2 * half,
+        ptr(q_weight), 0 if q_weight is None else code(q_weight),
+        ptr(k_weight), 0 if k_weight is None else code(k_weight),
+        0.0 if eps is None else eps, eps is not None, bool(interleaved), q_out.data_ptr(), ptr(k_out), *kv, *pages,
+        ptr(start), ptr(count), B, S, Hq, Hkv, D, _N.stream_of(dev))
+    status = _N.call_on(dev, _N.lib().mtp_qk_norm_rope, args)
+    if status:
+        _N.check(status, what)
     return q_out, k_out
 
 
@@ -523,37 +535,48 @@ def fused_qk_norm_rope_paged(
                          page_table, start, count, "fused_qk_norm_rope_paged")[0]
 
 
-def _window_attention(q4, out, k_pages, v_pages, page_table, seq_lens, q_lens, scale, window, sinks, key_weights,
-                      what):
-    B, S, Hq, D = q4
+@functools.lru_cache(maxsize=4096)
+def _window_workspace(dev, B, S, Hq, Hkv, D, width, window, sinks, code, weights):
+    return _N.call_on(dev, _N.lib().mtp_paged_window_attention_workspace, B, S, Hq, Hkv, D, width, window, sinks, code,
+                      weights)
+
+
+def _window_attention(q, B, S, Hq, D, k_pages, v_pages, page_table, seq_lens, q_lens, scale, window, sinks,
+                      key_weights, what):
+    q, k_pages, v_pages = q.contiguous(), k_pages.contiguous(), v_pages.contiguous()
+    page_table, seq_lens = _i32(page_table), _i32(seq_lens)
     P, Bp, Hkv, ps, Dp = k_pages.shape
-    assert (Bp, Dp) == (B, D) and v_pages.shape == k_pages.shape
-    assert k_pages.dtype == out.dtype and v_pages.dtype == out.dtype
-    assert Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}"
-    assert page_table.dim() == 2 and page_table.shape[0] == B and seq_lens.shape == (B,)
+    assert Bp == B and Dp == D and v_pages.shape == k_pages.shape
+    dtype = q.dtype
+    assert k_pages.dtype is dtype and v_pages.dtype is dtype, "q and the pools have one dtype"
+    assert Hkv > 0 and Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}"
+    assert page_table.dim() == 2, "page_table is [B, L]"
+    Bt, width = page_table.shape
+    assert Bt == B and seq_lens.shape == (B,)
     assert window is None or window > 0, "window is a positive number of positions, or None"
     assert sinks >= 0
-    width = page_table.shape[1]
+    if q_lens is not None:
+        q_lens = _i32(q_lens)
+        assert q_lens.shape == (B,)
     weight_ld = 0
     if key_weights is not None:
-        assert key_weights.dtype == torch.float32 and key_weights.is_contiguous(), "key_weights is added to in place"
-        assert key_weights.shape[:2] == (B, Hkv) and key_weights.dim() == 3 and key_weights.shape[2] >= width
-        weight_ld = key_weights.shape[2]
-    return B, S, Hq, Hkv, D, P, ps, width, weight_ld, (1.0 / math.sqrt(D) if scale is None else float(scale)), \
-        (0 if window is None else int(window))
-
-
-def _run_window_attention(q, out, k_pages, v_pages, page_table, seq_lens, q_lens, dims, sinks, key_weights, dev, what):
-    B, S, Hq, Hkv, D, P, ps, width, weight_ld, scale, window = dims
-    L, ptr, code = _N.lib(), _N.ptr, _N.dtype_code(q)
+        assert key_weights.dtype is torch.float32 and key_weights.is_contiguous(), "key_weights is added to in place"
+        Bw, Hw, weight_ld = key_weights.shape
+        assert Bw == B and Hw == Hkv and weight_ld >= width
+    dev = _N.same_device(q, k_pages, v_pages, page_table, seq_lens, q_lens, key_weights)
+    code, window = _N.dtype_code(q), 0 if window is None else int(window)
+    out = torch.empty_like(q)
     # scratch of this call alone: nothing is kept, and captured graphs share none
-    nbytes = _N.call_on(dev, L.mtp_paged_window_attention_workspace, B, S, Hq, Hkv, D, width, window, sinks, code,
-                        int(key_weights is not None))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _N.check(_N.call_on(
-        dev, L.mtp_paged_window_attention, ptr(q), ptr(k_pages), ptr(v_pages), ptr(page_table), width, ptr(seq_lens),
-        ptr(q_lens), ptr(out), code, B, S, Hq, Hkv, D, P, ps, scale, window, sinks, ptr(key_weights), weight_ld,
-        ptr(ws), nbytes, _N.stream_handle(dev)), what)
+    nbytes = _window_workspace(dev, B, S, Hq, Hkv, D, width, window, sinks, code, int(key_weights is not None))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    ptr = _N.address
+    args = _N.WINDOW_ATTENTION_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), width, seq_lens.data_ptr(),
+        ptr(q_lens), out.data_ptr(), code, B, S, Hq, Hkv, D, P, ps, 1.0 / math.sqrt(D) if scale is None else scale,
+        window, sinks, ptr(key_weights), weight_ld, ws.data_ptr(), nbytes, _N.stream_of(dev))
+    status = _N.call_on(dev, _N.lib().mtp_paged_window_attention, args)
+    if status:
+        _N.check(status, what)
     return out
 
 
@@ -573,16 +596,9 @@ def fused_paged_prompt_attention(
     ``window``, p - j < window or j < ``sinks``.  Returns [B,S,Hq,D] in q.dtype;
     rows behind q_lens are zero.  Cache positions that no row of the call sees
     may hold anything, their page-table entries too."""
-    q, k_pages, v_pages = q.contiguous(), k_pages.contiguous(), v_pages.contiguous()
-    page_table, seq_lens = _i32(page_table), _i32(seq_lens)
-    if q_lens is not None:
-        q_lens = _i32(q_lens)
-        assert q_lens.shape == (q.shape[0],)
-    dims = _window_attention(q.shape, q, k_pages, v_pages, page_table, seq_lens, q_lens, scale, window, sinks, None,
-                             "fused_paged_prompt_attention")
-    dev = _N.require_cuda(q, k_pages, v_pages, page_table, seq_lens, q_lens)
-    return _run_window_attention(q, torch.empty_like(q), k_pages, v_pages, page_table, seq_lens, q_lens, dims, sinks,
-                                 None, dev, "fused_paged_prompt_attention")
+    B, S, Hq, D = q.shape
+    return _window_attention(q, B, S, Hq, D, k_pages, v_pages, page_table, seq_lens, q_lens, scale, window, sinks,
+                             None, "fused_paged_prompt_attention")
 
 
 def fused_paged_decode_attention(
@@ -599,14 +615,9 @@ def fused_paged_decode_attention(
     float32 (optional): every visible key's softmax weight, summed over the
     query heads that share it, is added in place -- the totals that
     ``paged_kv_evict`` goes by.  Returns [B,Hq,D] in q.dtype."""
-    q, k_pages, v_pages = q.contiguous(), k_pages.contiguous(), v_pages.contiguous()
-    page_table, seq_lens = _i32(page_table), _i32(seq_lens)
     B, Hq, D = q.shape
-    dims = _window_attention((B, 1, Hq, D), q, k_pages, v_pages, page_table, seq_lens, None, scale, window, sinks,
+    return _window_attention(q, B, 1, Hq, D, k_pages, v_pages, page_table, seq_lens, None, scale, window, sinks,
                              key_weights, "fused_paged_decode_attention")
-    dev = _N.require_cuda(q, k_pages, v_pages, page_table, seq_lens, key_weights)
-    return _run_window_attention(q, torch.empty_like(q), k_pages, v_pages, page_table, seq_lens, None, dims, sinks,
-                                 key_weights, dev, "fused_paged_decode_attention")
 
 
 def paged_kv_evict(
@@ -628,24 +639,32 @@ def paged_kv_evict(
     assert k_pages.is_contiguous() and v_pages.is_contiguous(), "page pools are changed in place"
     assert key_weights.dtype == torch.float32 and key_weights.is_contiguous(), "key_weights is changed in place"
     P, B, Hkv, ps, D = k_pages.shape
-    assert v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype
+    assert v_pages.shape == k_pages.shape and v_pages.dtype is k_pages.dtype
     page_table, seq_lens = _i32(page_table), _i32(seq_lens)
-    assert page_table.dim() == 2 and page_table.shape[0] == B and seq_lens.shape == (B,)
-    assert key_weights.dim() == 3 and key_weights.shape[:2] == (B, Hkv)
-    assert key_weights.shape[2] >= page_table.shape[1]
+    Bt, width = page_table.shape
+    assert key_weights.dim() == 3, "key_weights is [B, Hkv, L]"
+    Bw, Hw, weight_ld = key_weights.shape
+    assert Bt == B and seq_lens.shape == (B,) and Bw == B and Hw == Hkv and weight_ld >= width
     assert budget >= 0 and sinks >= 0 and recent >= 0 and sinks + recent <= budget, \
         f"sinks={sinks} and recent={recent} do not fit budget={budget}"
-    dev = _N.require_cuda(k_pages, v_pages, page_table, seq_lens, key_weights)
-    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
-    L, ptr = _N.lib(), _N.ptr
-    nbytes = L.mtp_paged_kv_evict_workspace(B, Hkv, budget)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _N.check(_N.call_on(
-        dev, L.mtp_paged_kv_evict, ptr(k_pages), ptr(v_pages), _N.dtype_code(k_pages), ptr(page_table),
-        page_table.shape[1], P, ps, ptr(seq_lens), ptr(key_weights), key_weights.shape[2], ptr(kept), ptr(new_lens),
-        B, Hkv, D, int(budget), int(sinks), int(recent), ptr(ws), nbytes, _N.stream_handle(dev)), "paged_kv_evict")
+    dev = _N.same_device(k_pages, v_pages, page_table, seq_lens, key_weights)
+    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_pages.device)
+    new_lens = torch.empty_like(seq_lens)
+    nbytes = _evict_workspace(B, Hkv, budget)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=k_pages.device)
+    args = _N.KV_EVICT_ARGS.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), _N.dtype_code(k_pages), page_table.data_ptr(), width, P, ps,
+        seq_lens.data_ptr(), key_weights.data_ptr(), weight_ld, kept.data_ptr(), new_lens.data_ptr(), B, Hkv, D,
+        budget, sinks, recent, ws.data_ptr(), nbytes, _N.stream_of(dev))
+    status = _N.call_on(dev, _N.lib().mtp_paged_kv_evict, args)
+    if status:
+        _N.check(status, "paged_kv_evict")
     return kept, new_lens
+
+
+@functools.lru_cache(maxsize=4096)
+def _evict_workspace(B, H, budget):
+    return _N.lib().mtp_paged_kv_evict_workspace(B, H, budget)
 
 
 def fused_int4_matmul(

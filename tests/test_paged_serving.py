@@ -2,7 +2,6 @@
 sizes, dtypes, pointers and workspaces on the host before any launch, and the
 Python operators check shapes, strides, dtypes and devices.  CPU only."""
 
-import ctypes
 import math
 
 import pytest
@@ -11,7 +10,7 @@ import torch
 import paged_reference as R
 
 OK, SHAPE, DTYPE, WORKSPACE, ARG = 0, 1, 2, 6, 8
-P = ctypes.c_void_p(256)  # never dereferenced: every call below returns before a launch
+P = 256  # an address that is never dereferenced: every call below returns before a launch
 
 
 def rope_args(**kw):
@@ -21,7 +20,7 @@ def rope_args(**kw):
              count=None, B=2, S=3, Hq=4, Hkv=2, D=64, stream=None)
     assert set(kw) <= set(a)
     a.update(kw)
-    return list(a.values())
+    return [0 if x is None else x for x in a.values()]
 
 
 def attn_args(**kw):
@@ -30,7 +29,7 @@ def attn_args(**kw):
              stream=None)
     assert set(kw) <= set(a)
     a.update(kw)
-    return list(a.values())
+    return [0 if x is None else x for x in a.values()]
 
 
 def evict_args(**kw):
@@ -38,7 +37,7 @@ def evict_args(**kw):
              new_lens=P, B=2, H=2, D=64, budget=10, sinks=1, recent=2, ws=P, ws_bytes=1 << 40, stream=None)
     assert set(kw) <= set(a)
     a.update(kw)
-    return list(a.values())
+    return [0 if x is None else x for x in a.values()]
 
 
 PAGED = dict(k_pages=P, v_pages=P, table=P, stride=64, pages=8, ps=16, start=P)
@@ -55,7 +54,7 @@ PAGED = dict(k_pages=P, v_pages=P, table=P, stride=64, pages=8, ps=16, start=P)
 def test_rope_entry_refuses(kw, status):
     import _mtp_native as N
     before = N.lib().mtp_launch_count()
-    assert N.lib().mtp_qk_norm_rope(*rope_args(**kw)) == status
+    assert N.lib().mtp_qk_norm_rope(N.QK_NORM_ROPE_ARGS.pack(*rope_args(**kw))) == status
     assert N.lib().mtp_launch_count() == before
 
 
@@ -63,7 +62,7 @@ def test_rope_entry_refuses(kw, status):
     (dict(B=0), OK), (dict(S=0), OK), (dict(D=0), SHAPE), (dict(D=264), SHAPE), (dict(Hq=5), SHAPE),
     (dict(Hkv=0), SHAPE), (dict(ps=0), SHAPE), (dict(window=-1), SHAPE), (dict(sinks=-1), SHAPE),
     (dict(dtype=3), DTYPE), (dict(q=None), ARG), (dict(lens=None), ARG), (dict(table=None), ARG), (dict(k=None), ARG),
-    (dict(ws=None), WORKSPACE), (dict(ws_bytes=16), WORKSPACE), (dict(ws=ctypes.c_void_p(264)), WORKSPACE),
+    (dict(ws=None), WORKSPACE), (dict(ws_bytes=16), WORKSPACE), (dict(ws=264), WORKSPACE),
     (dict(weights=P, weight_ld=64), SHAPE),  # key weights with three rows a sequence
     (dict(weights=P, weight_ld=63, S=1), SHAPE), (dict(pages=1 << 31), SHAPE), (dict(stride=1 << 31), SHAPE),
     (dict(B=1 << 30), SHAPE),
@@ -71,7 +70,7 @@ def test_rope_entry_refuses(kw, status):
 def test_attention_entry_refuses(kw, status):
     import _mtp_native as N
     before = N.lib().mtp_launch_count()
-    assert N.lib().mtp_paged_window_attention(*attn_args(**kw)) == status
+    assert N.lib().mtp_paged_window_attention(N.WINDOW_ATTENTION_ARGS.pack(*attn_args(**kw))) == status
     assert N.lib().mtp_launch_count() == before
 
 
@@ -84,8 +83,44 @@ def test_attention_entry_refuses(kw, status):
 def test_evict_entry_refuses(kw, status):
     import _mtp_native as N
     before = N.lib().mtp_launch_count()
-    assert N.lib().mtp_paged_kv_evict(*evict_args(**kw)) == status
+    assert N.lib().mtp_paged_kv_evict(N.KV_EVICT_ARGS.pack(*evict_args(**kw))) == status
     assert N.lib().mtp_launch_count() == before
+
+
+def test_null_arguments_are_refused():
+    import _mtp_native as N
+    for f in (N.lib().mtp_qk_norm_rope, N.lib().mtp_paged_window_attention, N.lib().mtp_paged_kv_evict):
+        assert f(None) == ARG
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    """The packed structs have the sizes and member offsets that a C compiler
+    gives the header's."""
+    import os
+    import re
+    import shutil
+    import subprocess
+    import _mtp_native as N
+    from conftest import REPO
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    header = open(os.path.join(REPO, "include", "mtp_b200.h")).read()
+    src = '#include <stddef.h>\n#include <stdio.h>\n#include "mtp_b200.h"\nint main(void) {\n'
+    names = {"mtp_qk_norm_rope_args": N.QK_NORM_ROPE_ARGS, "mtp_paged_window_attention_args": N.WINDOW_ATTENTION_ARGS,
+             "mtp_paged_kv_evict_args": N.KV_EVICT_ARGS}
+    for name in names:
+        src += f'  printf("%zu %zu\\n", sizeof({name}), offsetof({name}, stream));\n'
+    src += "  return 0;\n}\n"
+    (tmp_path / "s.c").write_text(src)
+    subprocess.run([cc, "-std=c99", "-I", os.path.join(REPO, "include"), str(tmp_path / "s.c"), "-o",
+                    str(tmp_path / "s")], check=True)
+    out = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()
+    for i, (name, packed) in enumerate(names.items()):
+        assert int(out[2 * i]) == packed.size and int(out[2 * i + 1]) == packed.size - 8, name
+        body = re.search(r"typedef struct \{([^}]*)\} " + name, header).group(1)
+        doubles = [d for d in re.findall(r"double (\w+);", body)]
+        assert packed.format.replace("=", "").count("d") == len(doubles)
 
 
 def tensors():
