@@ -43,9 +43,9 @@ int launch_rope_vec(const rope::Args& a, int lph, unsigned gx, unsigned gy, cuda
 #define MTP_ROPE(L)                                                                              \
   (a.interleaved ? rope::qk_norm_rope_kernel<T, L, true><<<dim3(gx, gy), rope::kThreads, 0, s>>>(a) \
                  : rope::qk_norm_rope_kernel<T, L, false><<<dim3(gx, gy), rope::kThreads, 0, s>>>(a))
-  if (lph == 8) MTP_ROPE(8);
-  else if (lph == 16) MTP_ROPE(16);
-  else MTP_ROPE(32);
+  if (lph == 4) MTP_ROPE(4);
+  else if (lph == 8) MTP_ROPE(8);
+  else MTP_ROPE(16);
 #undef MTP_ROPE
   MTP_LAUNCH_CHECK();
   return MTP_OK;
@@ -268,7 +268,9 @@ int mtp_qk_norm_rope(const mtp_qk_norm_rope_args* args) {
   if (rot_dim % 2 != 0 || rot_dim > D)
     return fail(MTP_ERR_SHAPE, "rotated size %lld is odd or above the head size %lld", (long long)rot_dim,
                 (long long)D);
-  if (paged && (page_size <= 0 || num_pages < 0 || table_stride < 0)) return fail(MTP_ERR_SHAPE, "bad page sizes");
+  if (paged && (page_size <= 0 || num_pages < 0 || table_stride < 0 || page_size > INT32_MAX ||
+                table_stride > INT32_MAX))
+    return fail(MTP_ERR_SHAPE, "bad page sizes");
   if (!valid_dtype(dtype) || dtype == MTP_DTYPE_E4M3) return fail(MTP_ERR_DTYPE, "unsupported dtype %d", dtype);
   if ((q_weight && (!valid_dtype(q_weight_dtype) || q_weight_dtype == MTP_DTYPE_E4M3)) ||
       (k_weight && (!valid_dtype(k_weight_dtype) || k_weight_dtype == MTP_DTYPE_E4M3)))
@@ -310,7 +312,7 @@ int mtp_qk_norm_rope(const mtp_qk_norm_rope_args* args) {
   a.page_table = page_table;
   a.table_stride = table_stride;
   a.num_pages = num_pages;
-  a.page_size = page_size;
+  a.page_size = (int)page_size;
   a.start = paged ? start : nullptr;
   a.count = g.count;
   a.B = (int)B;
@@ -337,10 +339,12 @@ int mtp_qk_norm_rope(const mtp_qk_norm_rope_args* args) {
     MTP_LAUNCH_CHECK();
     return MTP_OK;
   }
-  const int lph = D <= 64 ? 8 : (D <= 128 ? 16 : 32);
+  for (int i = 0; i < 2; ++i) a.w_vec[i] = a.w[i] && a.w_dtype[i] == dtype && aligned16(a.w[i]);
+  const int lph = D <= 64 ? 4 : (D <= 128 ? 8 : 16);
   const int groups = rope::kThreads / lph, sms = sm_count(dev);
-  // eight tokens to a block once that still fills the GPU twice, else one token and its heads over several blocks
-  a.tokens = S >= 8 && B * ((S + 7) / 8) >= 2 * sms ? 8 : 1;
+  // Several tokens to a block once those blocks fill the GPU (a group's set-up
+  // then serves more heads), else one token and its heads over several blocks.
+  a.tokens = S >= 16 && B * ((S + 15) / 16) >= 4 * sms ? 16 : (S >= 8 && B * ((S + 7) / 8) >= 2 * sms ? 8 : 1);
   const int64_t gx = B * ((S + a.tokens - 1) / a.tokens);
   const int64_t most = (heads + groups / a.tokens - 1) / (groups / a.tokens);
   int64_t gy = (2 * sms + gx - 1) / gx;
