@@ -342,10 +342,12 @@ int mtp_qk_norm_rope(const mtp_qk_norm_rope_args* args) {
   for (int i = 0; i < 2; ++i) a.w_vec[i] = a.w[i] && a.w_dtype[i] == dtype && aligned16(a.w[i]);
   const int lph = D <= 64 ? 4 : (D <= 128 ? 8 : 16);
   const int groups = rope::kThreads / lph, sms = sm_count(dev);
-  // Several tokens to a block once those blocks fill the GPU (a group's set-up
-  // then serves more heads), else one token and its heads over several blocks.
-  a.tokens = S >= 16 && B * ((S + 15) / 16) >= 4 * sms ? 16 : (S >= 8 && B * ((S + 7) / 8) >= 2 * sms ? 8 : 1);
-  const int64_t gx = B * ((S + a.tokens - 1) / a.tokens);
+  // As many tokens to a block as bring the call down to one round of two blocks
+  // per SM (a group's set-up then serves more heads), 16 at most; where one
+  // token each leaves SMs without a block, its heads go over several blocks.
+  a.tokens = 1;
+  while (a.tokens < 16 && (B * S + a.tokens - 1) / a.tokens > 2 * sms) a.tokens *= 2;
+  const int64_t gx = (B * S + a.tokens - 1) / a.tokens;
   const int64_t most = (heads + groups / a.tokens - 1) / (groups / a.tokens);
   int64_t gy = (2 * sms + gx - 1) / gx;
   gy = gy < 1 ? 1 : (gy > most ? most : gy);
