@@ -187,6 +187,47 @@ __device__ __forceinline__ void fill_tokens(uint8_t* dst, const uint8_t* pool, c
   }
 }
 
+// One lane of the warp, the same one for every later use.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t lead;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(lead));
+  return lead;
+}
+
+// umma_f16, umma_f16_ts and umma_commit of a whole warp, issued by the lane with lead != 0
+__device__ __forceinline__ void umma_f16_lead(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts_lead(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                                 uint32_t accumulate, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_lead(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
 // AB_FMT: 1 = bf16, 0 = f16; DP: 64 or 128, the head size of the tiles (64 <=
 // D <= DP; the dimensions past D arrive as zeros)
 template <int AB_FMT, int DP>
@@ -217,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   static_assert((2 + 2 * kNumBuf + 2 + 4 + 2 + 2 * kIdRing + 1) * 8 + 8 <= 512, "barrier area");
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -247,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int ppc = p.slab > 0 ? kChunk / p.slab : 0;  // page slabs per chunk
 
   if (warp >= 8) {  // warpgroup 2: producer, MMA, page table, idle
@@ -381,83 +422,99 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&ids_full[slot]);
         }
       }
-    } else if (warp == kWarpMma && lane == 0) {
+    } else if (warp == kWarpMma) {
       // -------------------------------------------------------------- MMA issuer
-      int buffer = 0, queries = 0;
-      int done[2] = {0, 0};  // chunks of each tile so far
-      auto wait_buffer = [&](int k) -> bool {
-        return mbar_wait(&buf_full[k % kNumBuf], (k / kNumBuf) & 1, abort_flag);
+      // The whole warp walks the loop and one elected lane issues: with every
+      // value the same in all lanes, descriptors and addresses stay in uniform
+      // registers (issued from a one-lane branch a product took ~90 cycles of
+      // this warp, above the 64 it takes the tensor pipe).
+      const uint32_t lead = elect_one();
+      const uint64_t q_desc = sw128_kmajor_desc(smem_u32(sQ));
+      const uint64_t k_desc = sw128_kmajor_desc(smem_u32(sBuf));
+      const uint64_t v_desc = sw128_mnmajor_desc(smem_u32(sBuf), kHalfBytes);
+      int buf = 0;                    // ring buffer of the current K
+      uint32_t phase = 0;             // and its parity
+      uint32_t q_phase = 0;
+      uint32_t p_phase[2] = {0, 0};  // parity of each tile's next P
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool got = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+        tc_fence_after();
+        return got;
       };
+      auto after = [&](int k, int n) { return k + n >= kNumBuf ? k + n - kNumBuf : k + n; };
       auto issue_s = [&](int t, int k) {
         const uint32_t d = tmem_base + (uint32_t)(t * 128);
-        const uint32_t qa = smem_u32(sQ + t * kTileBytes), ka = smem_u32(sBuf + (k % kNumBuf) * kTileBytes);
+        const uint64_t qa = q_desc + (uint64_t)(t * (kTileBytes >> 4)), ka = k_desc + (uint64_t)(k * (kTileBytes >> 4));
 #pragma unroll
         for (int x = 0; x < DP / 16; ++x) {
-          const uint32_t off = (x >> 2) * kHalfBytes + (x & 3) * 32;
-          umma_f16(d, sw128_kmajor_desc(qa + off), sw128_kmajor_desc(ka + off), IDESC_S, x > 0);
+          const uint32_t off = ((x >> 2) * kHalfBytes + (x & 3) * 32) >> 4;
+          umma_f16_lead(d, qa + off, ka + off, IDESC_S, x > 0, lead);
         }
-        umma_commit(&s_full[t]);
+        umma_commit_lead(&s_full[t], lead);
       };
       // O_t += P_t V for keys [64 * half, 64 * half + 64) of the chunk
       auto issue_pv = [&](int t, int k, int half, bool acc) {
         const uint32_t d = tmem_base + (uint32_t)(256 + t * 128);
         const uint32_t pa = tmem_base + (uint32_t)(t * 128);
-        const uint32_t va = smem_u32(sBuf + (k % kNumBuf) * kTileBytes);
+        const uint64_t va = v_desc + (uint64_t)(k * (kTileBytes >> 4));
 #pragma unroll
         for (int x = 4 * half; x < 4 * half + 4; ++x)
-          umma_f16_ts(d, pa + x * 8, sw128_mnmajor_desc(va + x * 16 * 128, kHalfBytes), IDESC_PV,
-                      (acc || x > 0) ? 1u : 0u);
+          umma_f16_ts_lead(d, pa + x * 8, va + (uint64_t)((x * 16 * 128) >> 4), IDESC_PV, (acc || x > 0) ? 1u : 0u,
+                           lead);
       };
       for (int r = 0; ok; ++r) {
         const int index = item_index(p, r, &more);
         if (!more) break;
         if (index < 0) continue;
         const Item it = item_of(p, index);
-        const int n_it = it.count();
+        const int n0 = __shfl_sync(0xffffffffu, it.n_it[0], 0), n1 = __shfl_sync(0xffffffffu, it.n_it[1], 0);
+        const int n_it = max(n0, n1);
         if (n_it == 0) continue;
-        if (!(ok = mbar_wait(q_full, queries & 1, abort_flag))) break;
-        ++queries;
-        if (!(ok = wait_buffer(buffer))) break;
-        tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (it.n_it[t] > 0) issue_s(t, buffer);
-        umma_commit(&buf_empty[buffer % kNumBuf]);
-        if (n_it == 1) umma_commit(q_empty);
-        for (int i = 0; i < n_it && ok; ++i, buffer += 2) {
-          const int v = buffer + 1, knext = buffer + 2;
-          const int t_first = i < it.n_it[0] ? 0 : 1;                                  // tiles that take chunk i
-          const int t_last = i < it.n_it[1] ? 1 : 0;
-          const int s_first = i + 1 < it.n_it[0] ? 0 : 1, s_last = i + 1 < it.n_it[1] ? 1 : 0;  // and chunk i + 1
-          for (int t = t_first; t <= t_last && ok; ++t) {
-            if (!(ok = mbar_wait(&p_full[2 * t], done[t] & 1, abort_flag))) break;
-            tc_fence_after();
-            if (t == t_first) {
-              if (!(ok = wait_buffer(v))) break;
-              tc_fence_after();
-            }
-            issue_pv(t, v, 0, i > 0);
-            if (!(ok = mbar_wait(&p_full[2 * t + 1], done[t] & 1, abort_flag))) break;
-            tc_fence_after();
-            issue_pv(t, v, 1, true);
-            umma_commit(&pv_done[t]);
-            ++done[t];
-            if (t == t_last) umma_commit(&buf_empty[v % kNumBuf]);
-            if (i + 1 < it.n_it[t]) {
-              if (t == s_first) {
-                if (!(ok = wait_buffer(knext))) break;
-                tc_fence_after();
+        if (!(ok = wait(q_full, q_phase))) break;
+        q_phase ^= 1u;
+        if (!(ok = wait(&buf_full[buf], phase))) break;
+        if (n0 > 0) issue_s(0, buf);
+        if (n1 > 0) issue_s(1, buf);
+        umma_commit_lead(&buf_empty[buf], lead);
+        if (n_it == 1) umma_commit_lead(q_empty, lead);
+#pragma unroll 1
+        for (int i = 0; i < n_it; ++i) {
+          const int v = after(buf, 1), next = after(buf, 2);
+          const uint32_t v_phase = phase ^ (v < buf ? 1u : 0u), next_phase = phase ^ (next < buf ? 1u : 0u);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int n_t = t == 0 ? n0 : n1;
+            if (i < n_t) {
+              if (!(ok = wait(&p_full[2 * t], p_phase[t]))) break;
+              if (t == 0 || i >= n0) {  // the first tile of the chunk
+                if (!(ok = wait(&buf_full[v], v_phase))) break;
               }
-              issue_s(t, knext);
-              if (t == s_last) {
-                umma_commit(&buf_empty[knext % kNumBuf]);
-                if (i + 2 == n_it) umma_commit(q_empty);
+              issue_pv(t, v, 0, i > 0);
+              if (!(ok = wait(&p_full[2 * t + 1], p_phase[t]))) break;
+              issue_pv(t, v, 1, true);
+              p_phase[t] ^= 1u;
+              if (i + 1 == n_t) umma_commit_lead(&pv_done[t], lead);
+              if (t == 1 || i >= n1) umma_commit_lead(&buf_empty[v], lead);  // the last tile of the chunk
+              if (i + 1 < n_t) {
+                if (t == 0 || i + 1 >= n0) {
+                  if (!(ok = wait(&buf_full[next], next_phase))) break;
+                }
+                issue_s(t, next);
+                if (t == 1 || i + 1 >= n1) {
+                  umma_commit_lead(&buf_empty[next], lead);
+                  if (i + 2 == n_it) umma_commit_lead(q_empty, lead);
+                }
               }
             }
           }
+          if (!ok) break;
+          buf = next;
+          phase = next_phase;
         }
       }
-      umma_commit(drain);
-      mbar_wait(drain, 0, abort_flag, /*honour_abort=*/false);
+      umma_commit_lead(drain, lead);
+      if (lane == 0) mbar_wait(drain, 0, abort_flag, /*honour_abort=*/false);
+      __syncwarp();
     }
   } else {  // warpgroups 0-1: softmax of query tiles 0 and 1
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -468,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + (uint32_t)(t * 128);
     const uint32_t o_addr = tmem_base + lane_off + (uint32_t)(256 + t * 128);
-    int done = 0;  // chunks of this tile so far
+    int done = 0, finished = 0;  // chunks and items of this tile so far
     bool ok = true, more = true;
     for (int r = 0; ok; ++r) {
       const int index = item_index(p, r, &more);
@@ -514,12 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                     attn::fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
         const float m_new = fmaxf(m_run, mx);
         if (i > 0) {
-          // P and O may be touched only after the previous PV completed
-          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], (done + i - 1) & 1, abort_flag))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+          // The scores of this chunk were issued after the last chunk's P V, so
+          // O and P's columns are free here without another wait.
           const bool need = m_new > m_run + attn::kRescaleThreshold;
           if (__any_sync(0xffffffffu, need)) {
             const float alpha = need ? attn::ex2(m_run - m_new) : 1.0f;
@@ -556,7 +609,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       done += n_it;
-      if (n_it > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[t], (done - 1) & 1, abort_flag))) break;
+      if (n_it > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], finished & 1, abort_flag))) break;
+        ++finished;
+      }
       tc_fence_after();
       if (p.splits == 1) {
         const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
