@@ -138,16 +138,7 @@ template <int AB_FMT, int DP>
 int launch_prompt_inst(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const prompt::Params& p,
                        int sms, int dev, cudaStream_t s) {
   static bool attr[kMaxDevices] = {};
-  static bool regs_ok[kMaxDevices] = {};
   constexpr int smem = prompt::smem_bytes(DP);
-  if (!regs_ok[dev]) {  // setmaxnreg moves registers inside the launch's reservation; with another one it could wait
-    cudaFuncAttributes fa;
-    MTP_CUDA_TRY(cudaFuncGetAttributes(&fa, prompt::prompt_attention_tc_kernel<AB_FMT, DP>));
-    if (fa.numRegs != prompt::kLaunchRegs)
-      return fail(MTP_ERR_CUDA, "prompt attention kernel reserves %d registers per thread, its register split needs %d",
-                  fa.numRegs, prompt::kLaunchRegs);
-    regs_ok[dev] = true;
-  }
   if (int st = set_smem_once(prompt::prompt_attention_tc_kernel<AB_FMT, DP>, smem, attr, dev)) return st;
   const unsigned grid = (unsigned)(p.items < sms ? p.items : sms);
   prompt::prompt_attention_tc_kernel<AB_FMT, DP><<<grid, prompt::kThreads, smem, s>>>(tq, tk, tv, p);

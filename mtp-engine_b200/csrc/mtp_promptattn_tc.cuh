@@ -7,20 +7,22 @@
 // An item is one (sequence, key head, pair of query tiles): a tile holds
 // tpt = 128 / G positions x G heads (row r = position * G + head), so a
 // 128-key chunk of K and V is read once for 256 rows.  Persistent: one block
-// of 384 threads per SM walks over the items, the ones with the most keys
+// of 576 threads per SM walks over the items, the ones with the most keys
 // first and every other round in reverse, which evens out causal lengths
-// without a counter in memory.  Roles as in tree_attention_tc_kernel, whose
-// inner loop this shares:
-//   warps 0-3, 4-7  softmax of tile 0 / 1, one row per thread: scores from
-//                   tensor memory, running maximum with lazy rescaling, P
-//                   (16-bit) back over the scores' first columns, the output
-//   warp 8          producer: Q of the item, then the chunks' K and V -- whole
-//                   page slabs by TMA, or token by token where a chunk's
-//                   table is not page-granular or where the chunk holds keys
-//                   that no row of the call may see (those are zero-filled:
-//                   their slots may hold anything, and 0 * NaN is NaN)
-//   warp 9          tcgen05.mma issuer
-//   warp 10         page-table reader, up to kIdRing chunks ahead
+// without a counter in memory.  Roles:
+//   warps 0-15  softmax, eight warps to a tile: four for the first 64 keys of a
+//               chunk and four for the last 64, one thread per row each.  Scores
+//               from tensor memory, the row's maximum exchanged between the two
+//               threads, lazy rescaling, P (16-bit) back over the scores, half of
+//               the output each.  With one thread per row (128 scores in its
+//               registers, two warps per SM sub-partition) the exponentials ran
+//               at half the rate of the exp2 unit.
+//   warp 16     producer: Q of the item, then the chunks' K and V -- whole
+//               page slabs by TMA, or token by token where a chunk's
+//               table is not page-granular or where the chunk holds keys
+//               that no row of the call may see (those are zero-filled:
+//               their slots may hold anything, and 0 * NaN is NaN)
+//   warp 17     tcgen05.mma issuer
 // All rings and barrier phases run on from item to item: the next item's keys
 // are already on their way, and its first scores are computed, while the
 // softmax warps write the last item's output.
@@ -40,18 +42,15 @@ namespace mtp {
 namespace prompt {
 
 using attn::kChunk;
-using attn::kIdRing;
-using attn::kLaunchRegs;
-using attn::kMaxPagesPerChunk;
-using attn::kRegsAux;
-using attn::kRegsSoftmax;
-using attn::kThreads;
+constexpr int kThreads = 576;  // 112 registers each
+constexpr int kSoftmaxWarps = 16;
+constexpr int kWarpProducer = 16, kWarpMma = 17;
 constexpr int kHalfBytes = 128 * 128;  // 128 rows x 64 dims
-constexpr int kWarpProducer = 8, kWarpMma = 9, kWarpTable = 10;
 constexpr int tile_bytes(int dp) { return dp / 64 * kHalfBytes; }
-constexpr int num_buf(int dp) { return dp == 128 ? 5 : 10; }  // 160 KB of K and V in flight
+constexpr int num_buf(int dp) { return dp == 128 ? 4 : 8; }  // 128 KB of K and V in flight
+constexpr int kExchangeBytes = 2 * 2 * 2 * 128 * 4;           // [turn][tile][half of the keys][row]
 constexpr int smem_bytes(int dp) {
-  return 2 * tile_bytes(dp) + num_buf(dp) * tile_bytes(dp) + kIdRing * kMaxPagesPerChunk * 4 + 512 + 1024;
+  return 2 * tile_bytes(dp) + num_buf(dp) * tile_bytes(dp) + kExchangeBytes + 256 + 1024;
 }
 static_assert(smem_bytes(128) <= 227 * 1024 && smem_bytes(64) <= 227 * 1024, "shared memory per CTA");
 
@@ -187,6 +186,49 @@ __device__ __forceinline__ void fill_tokens(uint8_t* dst, const uint8_t* pool, c
   }
 }
 
+// mbar_wait with its limit in clock cycles: reading the nanosecond timer on the
+// way into a wait costs hundreds of cycles, which here sit between one tile's P
+// and its next product.
+constexpr long long kWaitLimitCycles = 4000000000ll;  // about 2 s
+
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      *abort = 1;
+      record_error(MTP_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+// P of 16 scores: 2^(s * mul - m) packed as 16-bit pairs, with the running sums
+// in (ls0, ls1).
+template <int AB_FMT>
+__device__ __forceinline__ void exp_pack16(const uint32_t (&s)[16], float mul, float m_use, float& ls0, float& ls1,
+                                           uint32_t (&out)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float x0, x1;
+    attn::ffma2(x0, x1, __uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1]), mul, mul, -m_use, -m_use);
+    const float e0 = attn::ex2(x0), e1 = attn::ex2(x1);
+    attn::add2(ls0, ls1, e0, e1);
+    out[j] = attn::pack_bf16(e0, e1, AB_FMT == 1 ? MTP_DTYPE_BF16 : MTP_DTYPE_F16);
+  }
+}
+
+// 32 lanes x 8 consecutive 32-bit columns <- 8 registers per thread
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 // One lane of the warp, the same one for every later use.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t lead;
@@ -242,21 +284,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sBuf = sQ + 2 * kTileBytes;
-  int* sIds = reinterpret_cast<int*>(sBuf + kNumBuf * kTileBytes);  // [kIdRing][kMaxPagesPerChunk]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sIds + kIdRing * kMaxPagesPerChunk);
+  float* sExchange = reinterpret_cast<float*>(sBuf + kNumBuf * kTileBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sExchange) + kExchangeBytes);
   uint64_t* q_full = bars;
   uint64_t* q_empty = bars + 1;
   uint64_t* buf_full = bars + 2;
   uint64_t* buf_empty = buf_full + kNumBuf;
   uint64_t* s_full = buf_empty + kNumBuf;  // [2]
-  uint64_t* p_full = s_full + 2;           // [2 tiles][2 halves of 64 keys]
+  uint64_t* p_full = s_full + 2;           // [2 tiles][first 48 keys of each half, last 16]
   uint64_t* pv_done = p_full + 4;          // [2]
-  uint64_t* ids_full = pv_done + 2;        // [kIdRing]
-  uint64_t* ids_empty = ids_full + kIdRing;
-  uint64_t* drain = ids_empty + kIdRing;
+  uint64_t* drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 + 2 * kNumBuf + 2 + 4 + 2 + 2 * kIdRing + 1) * 8 + 8 <= 512, "barrier area");
+  static_assert((2 + 2 * kNumBuf + 2 + 4 + 2 + 1) * 8 + 8 <= 256, "barrier area");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -269,13 +309,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[2 * t], 4);  // one arrival per softmax warp
-      mbar_init(&p_full[2 * t + 1], 4);
+      mbar_init(&p_full[2 * t], 8);  // one arrival per softmax warp of the tile
+      mbar_init(&p_full[2 * t + 1], 8);
       mbar_init(&pv_done[t], 1);
-    }
-    for (int i = 0; i < kIdRing; ++i) {
-      mbar_init(&ids_full[i], 1);
-      mbar_init(&ids_empty[i], 1);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -291,8 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int ppc = p.slab > 0 ? kChunk / p.slab : 0;  // page slabs per chunk
 
-  if (warp >= 8) {  // warpgroup 2: producer, MMA, page table, idle
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsAux));
+  if (warp >= kSoftmaxWarps) {  // producer, MMA
     bool ok = true, more = true;
     if (warp == kWarpProducer) {
       // -------------------------------------------------------------- producer (whole warp)
@@ -301,7 +336,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
       }
-      int buffer = 0, chunks = 0, queries = 0;  // buffers, chunks and Q loads so far
+      int buffer = 0, queries = 0;  // buffers and Q loads so far
+      // Lane l reads the page ids of tokens 4 l .. 4 l + 3 of a chunk, one chunk
+      // ahead.  A chunk is page-granular if all tokens of every slab lie in the
+      // page of the slab's first one.
+      const int per_slab = p.slab > 0 ? p.slab / 4 : 1;  // lanes of a slab
+      int id[4];
+      auto read_ids = [&](const Item& it, int c) {
+        id[0] = id[1] = id[2] = id[3] = INT32_MIN;
+        if (p.slab > 0 && it.whole(p, c)) {  // then all 128 columns are inside the table
+          const int32_t* src = p.page_table + (int64_t)it.b * p.table_stride + c * kChunk + lane * 4;
+          if (p.table_vec) {
+            const int4 e = __ldg(reinterpret_cast<const int4*>(src));
+            id[0] = e.x, id[1] = e.y, id[2] = e.z, id[3] = e.w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) id[k] = __ldg(src + k);
+          }
+        }
+      };
       for (int r = 0; ok; ++r) {
         const int index = item_index(p, r, &more);
         if (!more) break;
@@ -309,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Item it = item_of(p, index);
         const int n_it = it.count();
         if (n_it == 0) continue;
+        read_ids(it, it.chunk(0));
         {
           bool got = true;
           if (lane == 0) {
@@ -325,20 +379,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++queries;
           if (!__shfl_sync(0xffffffffu, got, 0)) break;
         }
-        for (int i = 0; i < n_it && ok; ++i, ++chunks) {
+        for (int i = 0; i < n_it && ok; ++i) {
           const int c = it.chunk(i);
-          const int slot = chunks % kIdRing;
-          int pg = 0;
+          const int page = (int)resolve_page(id[0], p.num_pages);  // -1 where nothing was read
+          bool gran = page >= 0;
+#pragma unroll
+          for (int k = 1; k < 4; ++k) gran &= (int)resolve_page(id[k], p.num_pages) == page;
+          const int head = __shfl_sync(0xffffffffu, page, lane / per_slab * per_slab);
+          const bool per_token = !__all_sync(0xffffffffu, gran && head == page);
+          const int pg = __shfl_sync(0xffffffffu, page, (lane * per_slab) & 31);  // page of this lane's slab
+          if (i + 1 < n_it) read_ids(it, it.chunk(i + 1));
           bool got = true;
-          if (lane == 0) got = mbar_wait(&ids_full[slot], (chunks / kIdRing) & 1, abort_flag);
-          if (!__shfl_sync(0xffffffffu, got, 0)) {
-            ok = false;
-            break;
-          }
-          if (lane < ppc) pg = sIds[slot * kMaxPagesPerChunk + lane];
-          const bool per_token = sIds[slot * kMaxPagesPerChunk] < 0;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ids_empty[slot]);
           int rows[4];
           if (per_token) token_rows(p, it, c * kChunk, lane, rows);
           for (int kv = 0; kv < 2; ++kv, ++buffer) {
@@ -376,52 +427,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       attn::cp_async_wait_all();  // after an abort too: no copy of this warp may land after the block's end
-    } else if (warp == kWarpTable) {
-      // -------------------------------------------------------------- page-table warp
-      // Lane l looks at tokens 4 l .. 4 l + 3 of a chunk: page-granular if all
-      // tokens of every slab lie in the page of the slab's first one.
-      int chunks = 0;
-      for (int r = 0; ok; ++r) {
-        const int index = item_index(p, r, &more);
-        if (!more) break;
-        if (index < 0) continue;
-        const Item it = item_of(p, index);
-        const int n_it = it.count();
-        const int32_t* table = p.page_table + (int64_t)it.b * p.table_stride;
-        for (int i = 0; i < n_it; ++i, ++chunks) {
-          const int c = it.chunk(i);
-          const int slot = chunks % kIdRing;
-          int id[4] = {-1, -1, -1, -1};
-          const bool whole = p.slab > 0 && it.whole(p, c);  // then all 128 columns are inside the table
-          if (whole) {
-            const int32_t* src = table + c * kChunk + lane * 4;
-            if (p.table_vec) {
-              const int4 e = __ldg(reinterpret_cast<const int4*>(src));
-              id[0] = e.x, id[1] = e.y, id[2] = e.z, id[3] = e.w;
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) id[k] = __ldg(src + k);
-            }
-          }
-          bool got = true;
-          if (lane == 0) got = mbar_wait(&ids_empty[slot], ((chunks / kIdRing) & 1) ^ 1u, abort_flag);
-          if (!__shfl_sync(0xffffffffu, got, 0)) {
-            ok = false;
-            break;
-          }
-          const int page = whole ? (int)resolve_page(id[0], p.num_pages) : -1;
-          bool gran = page >= 0;
-#pragma unroll
-          for (int k = 1; k < 4; ++k) gran &= (int)resolve_page(id[k], p.num_pages) == page;
-          const int per_slab = p.slab > 0 ? p.slab / 4 : 1;  // lanes of a slab
-          const int head = __shfl_sync(0xffffffffu, page, lane / per_slab * per_slab);
-          gran = __all_sync(0xffffffffu, gran && head == page);
-          const int mine = __shfl_sync(0xffffffffu, page, (lane * per_slab) & 31);
-          if (lane < max(ppc, 1)) sIds[slot * kMaxPagesPerChunk + lane] = gran ? mine : -1;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ids_full[slot]);
-        }
-      }
     } else if (warp == kWarpMma) {
       // -------------------------------------------------------------- MMA issuer
       // The whole warp walks the loop and one elected lane issues: with every
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t q_phase = 0;
       uint32_t p_phase[2] = {0, 0};  // parity of each tile's next P
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        const bool got = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+        const bool got = __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag));
         tc_fence_after();
         return got;
       };
@@ -452,15 +457,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         umma_commit_lead(&s_full[t], lead);
       };
-      // O_t += P_t V for keys [64 * half, 64 * half + 64) of the chunk
-      auto issue_pv = [&](int t, int k, int half, bool acc) {
+      // O_t += P_t V for the first 48 keys of each half of the chunk (part 0), or their last 16
+      auto issue_pv = [&](int t, int k, int part, bool acc) {
         const uint32_t d = tmem_base + (uint32_t)(256 + t * 128);
         const uint32_t pa = tmem_base + (uint32_t)(t * 128);
         const uint64_t va = v_desc + (uint64_t)(k * (kTileBytes >> 4));
 #pragma unroll
-        for (int x = 4 * half; x < 4 * half + 4; ++x)
-          umma_f16_ts_lead(d, pa + x * 8, va + (uint64_t)((x * 16 * 128) >> 4), IDESC_PV, (acc || x > 0) ? 1u : 0u,
-                           lead);
+        for (int x = 0; x < 8; ++x)
+          if (((x & 3) == 3) == (part == 1))
+            umma_f16_ts_lead(d, pa + (x >> 2) * 64 + (x & 3) * 8, va + (uint64_t)((x * 16 * 128) >> 4), IDESC_PV, (acc || x > 0) ? 1u : 0u,
+                             lead);
       };
       for (int r = 0; ok; ++r) {
         const int index = item_index(p, r, &more);
@@ -516,15 +522,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_wait(drain, 0, abort_flag, /*honour_abort=*/false);
       __syncwarp();
     }
-  } else {  // warpgroups 0-1: softmax of query tiles 0 and 1
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const int t = warp / 4;
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int t = warp / 8, half = warp / 4 % 2;  // tile, half of the chunk's keys
     const int q = warp & 3;
     const int row = q * 32 + lane;  // row within the tile == TMEM lane
     const int row_s = row / p.G, g = row % p.G;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t s_addr = tmem_base + lane_off + (uint32_t)(t * 128);
-    const uint32_t o_addr = tmem_base + lane_off + (uint32_t)(256 + t * 128);
+    const uint32_t s_addr = tmem_base + lane_off + (uint32_t)(t * 128 + half * 64);  // this half's scores
+    const uint32_t p_addr = s_addr;  // and its P, over the first 32 of its 64 columns
+    const uint32_t o_addr = tmem_base + lane_off + (uint32_t)(256 + t * 128 + half * (DP / 2));  // half of the output
+    // the two warps that share 32 rows tell each other a value per row
+    float* const ex_mine = sExchange + (t * 2 + half) * 128 + row;
+    float* const ex_other = sExchange + (t * 2 + (half ^ 1)) * 128 + row;
+    int turn = 0;
+    auto exchange = [&](float v) -> float {
+      ex_mine[turn] = v;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + q) : "memory");
+      const float o = ex_other[turn];
+      turn ^= 2 * 2 * 128;  // the other set of slots next time: this one may still be being read
+      return o;
+    };
     int done = 0, finished = 0;  // chunks and items of this tile so far
     bool ok = true, more = true;
     for (int r = 0; ok; ++r) {
@@ -537,39 +555,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool row_ok = in_tile && s < it.n;
       const int pos = row_ok ? it.len - it.n + s : -1;
       const int lo = pos - p.window + 1;
-      const int n_it = it.n_it[t];
+      const int n_it = t == 0 ? it.n_it[0] : it.n_it[1];
       float m_run = -INFINITY, l_run = 0.f;
       for (int i = 0; i < n_it; ++i) {
-        const int first = it.chunk(i) * kChunk;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (done + i) & 1, abort_flag))) {
+        const int first = it.chunk(i) * kChunk + half * 64;
+        if (!__all_sync(0xffffffffu, wait_bar(&s_full[t], (done + i) & 1, abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const bool no_masked = first + kChunk - 1 <= pos && (first >= lo || first + kChunk <= p.sinks);
-        uint32_t sc[128];
+        const bool no_masked = first + 63 <= pos && (first >= lo || first + 64 <= p.sinks);
+        // four blocks of 16 scores and, later, of 8 registers of P: larger
+        // blocks of consecutive registers cost spills
+        uint32_t sc[4][16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) tmem_ld32(s_addr + j * 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[32 * j]));
+        for (int k = 0; k < 4; ++k) tmem_ld16(s_addr + 16 * k, sc[k]);
         tmem_wait_ld();
         if (!no_masked) {
-          uint32_t mw[4];
+          const uint32_t mw[2] = {mask_word(first, pos, lo, p.sinks), mask_word(first + 32, pos, lo, p.sinks)};
 #pragma unroll
-          for (int w = 0; w < 4; ++w) mw[w] = mask_word(first + 32 * w, pos, lo, p.sinks);
-#pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if (!((mw[j >> 5] >> (j & 31)) & 1u)) sc[j] = 0xff800000u;  // -inf
+          for (int j = 0; j < 64; ++j)
+            if (!((mw[j >> 5] >> (j & 31)) & 1u)) sc[j >> 4][j & 15] = 0xff800000u;  // -inf
         }
-        float m8[8];
+        float m4[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(sc[k]), __uint_as_float(sc[k + 8]));
+        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(__uint_as_float(sc[k][0]), __uint_as_float(sc[k][1]));
 #pragma unroll
-        for (int j = 16; j < 128; j += 16)
+        for (int j = 2; j < 16; j += 2)
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            m8[k] = attn::fmax3(m8[k], __uint_as_float(sc[j + k]), __uint_as_float(sc[j + 8 + k]));
-        const float mx = p.scale_log2 * attn::fmax3(attn::fmax3(m8[0], m8[1], m8[2]),
-                                                    attn::fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-        const float m_new = fmaxf(m_run, mx);
+          for (int k = 0; k < 4; ++k)
+            m4[k] = attn::fmax3(m4[k], __uint_as_float(sc[k][j]), __uint_as_float(sc[k][j + 1]));
+        const float mx = p.scale_log2 * fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        // both halves go by the greater maximum
+        const float m_new = attn::fmax3(m_run, mx, exchange(mx));
         if (i > 0) {
           // The scores of this chunk were issued after the last chunk's P V, so
           // O and P's columns are free here without another wait.
@@ -577,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (__any_sync(0xffffffffu, need)) {
             const float alpha = need ? attn::ex2(m_run - m_new) : 1.0f;
 #pragma unroll 1
-            for (int j = 0; j < DP / 16; ++j) {
+            for (int j = 0; j < DP / 32; ++j) {
               uint32_t o[16];
               tmem_ld16(o_addr + j * 16, o);
               tmem_wait_ld();
@@ -595,35 +613,62 @@ __global__ void __launch_bounds__(kThreads, 1)
           m_run = m_new;
         }
         const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+        // P in two parts, 48 keys and 16: only a quarter of P V is left to do
+        // once the last part is there
         float ls0 = 0.f, ls1 = 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          attn::exp_pack_half<AB_FMT>(sc, h, p.scale_log2, m_use, ls0, ls1);
-          tmem_st32(s_addr + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(&sc[32 * h]));
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
+        {
+          uint32_t pk[8];
+          exp_pack16<AB_FMT>(sc[0], p.scale_log2, m_use, ls0, ls1, pk);
+          tmem_st8(p_addr, pk);
         }
+        {
+          uint32_t pk[8];
+          exp_pack16<AB_FMT>(sc[1], p.scale_log2, m_use, ls0, ls1, pk);
+          tmem_st8(p_addr + 8, pk);
+        }
+        {
+          uint32_t pk[8];
+          exp_pack16<AB_FMT>(sc[2], p.scale_log2, m_use, ls0, ls1, pk);
+          tmem_st8(p_addr + 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t]);
+        {
+          uint32_t pk[8];
+          exp_pack16<AB_FMT>(sc[3], p.scale_log2, m_use, ls0, ls1, pk);
+          tmem_st8(p_addr + 24, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + 1]);
         l_run += ls0 + ls1;
       }
       if (!ok) break;
       done += n_it;
       if (n_it > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], finished & 1, abort_flag))) break;
+        l_run += exchange(l_run);
+        if (!__all_sync(0xffffffffu, wait_bar(&pv_done[t], finished & 1, abort_flag))) break;
         ++finished;
+        tc_fence_after();
       }
-      tc_fence_after();
+      constexpr int kCols = DP / 2;  // this half's columns of the output
+      const int col0 = half * kCols;
       if (p.splits == 1) {
         const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
         uint8_t* orow = static_cast<uint8_t*>(p.out) +
-                        ((((int64_t)it.b * p.S + s) * p.Hq + (int64_t)it.kvh * p.G + g) * p.D) * 2;
+                        ((((int64_t)it.b * p.S + s) * p.Hq + (int64_t)it.kvh * p.G + g) * p.D + col0) * 2;
 #pragma unroll 1
-        for (int j = 0; j < DP / 32; ++j) {
+        for (int j = 0; j < kCols / 32; ++j) {
           uint32_t o[32];
           if (n_it > 0) {
             tmem_ld32(o_addr + j * 32, o);
             tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0u;
           }
           if (in_tile) {
             uint32_t w[16];
@@ -635,14 +680,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint4* dst = reinterpret_cast<uint4*>(orow + j * 64);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (j * 32 + k * 8 < p.D) dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+              if (col0 + j * 32 + k * 8 < p.D)
+                dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
           }
         }
       } else if (n_it > 0 || row_ok) {
         const int64_t slot = (int64_t)index * 256 + t * 128 + row;
-        float* po = p.part_o + slot * p.D;
+        float* po = p.part_o + slot * p.D + col0;
 #pragma unroll 1
-        for (int j = 0; j < (n_it > 0 ? DP / 32 : 0); ++j) {
+        for (int j = 0; j < (n_it > 0 ? kCols / 32 : 0); ++j) {
           uint32_t o[32];
           tmem_ld32(o_addr + j * 32, o);
           tmem_wait_ld();
@@ -650,12 +696,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             float4* dst = reinterpret_cast<float4*>(po + j * 32);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              if (j * 32 + k * 4 < p.D)
+              if (col0 + j * 32 + k * 4 < p.D)
                 dst[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
                                      __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
           }
         }
-        if (row_ok) {
+        if (row_ok && half == 0) {
           p.part_ml[slot * 2] = m_run;  // -inf: no key of this piece is visible, and its output is not read
           p.part_ml[slot * 2 + 1] = l_run;
         }
