@@ -7,7 +7,7 @@
 // An item is one (sequence, key head, pair of query tiles): a tile holds
 // tpt = 128 / G positions x G heads (row r = position * G + head), so a
 // 128-key chunk of K and V is read once for 256 rows.  Persistent: one block
-// of 576 threads per SM walks over the items, the ones with the most keys
+// of 640 threads per SM walks over the items, the ones with the most keys
 // first and every other round in reverse, which evens out causal lengths
 // without a counter in memory.  Roles:
 //   warps 0-15  softmax, eight warps to a tile: four for the first 64 keys of a
@@ -17,11 +17,12 @@
 //               the output each.  With one thread per row (128 scores in its
 //               registers, two warps per SM sub-partition) the exponentials ran
 //               at half the rate of the exp2 unit.
-//   warp 16     producer: Q of the item, then the chunks' K and V -- whole
-//               page slabs by TMA, or token by token where a chunk's
-//               table is not page-granular or where the chunk holds keys
-//               that no row of the call may see (those are zero-filled:
-//               their slots may hold anything, and 0 * NaN is NaN)
+//   warps 16, 18  producers of Q and K, and of V: whole page slabs by TMA, or
+//               token by token where a chunk's table is not page-granular or
+//               where the chunk holds keys that no row of the call may see
+//               (those are zero-filled: their slots may hold anything, and
+//               0 * NaN is NaN).  Two warps because a page load takes one of
+//               them 100 cycles and more, 32 loads a chunk with 16-token pages
 //   warp 17     tcgen05.mma issuer
 // All rings and barrier phases run on from item to item: the next item's keys
 // are already on their way, and its first scores are computed, while the
@@ -42,9 +43,9 @@ namespace mtp {
 namespace prompt {
 
 using attn::kChunk;
-constexpr int kThreads = 576;  // 112 registers each
+constexpr int kThreads = 640;  // 96 registers each
 constexpr int kSoftmaxWarps = 16;
-constexpr int kWarpProducer = 16, kWarpMma = 17;
+constexpr int kWarpK = 16, kWarpMma = 17, kWarpV = 18;
 constexpr int kHalfBytes = 128 * 128;  // 128 rows x 64 dims
 constexpr int tile_bytes(int dp) { return dp / 64 * kHalfBytes; }
 constexpr int num_buf(int dp) { return dp == 128 ? 4 : 8; }  // 128 KB of K and V in flight
@@ -229,45 +230,22 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                : "memory");
 }
 
-// One lane of the warp, the same one for every later use.
-__device__ __forceinline__ uint32_t elect_one() {
+// True in one lane of a converged warp.  Products, commits and page loads are
+// issued as `if (elect_one()) { ... } __syncwarp();`: the branch tells the
+// compiler that one lane is active, so operands go through uniform registers,
+// and the other lanes wait behind it -- those registers belong to the whole
+// warp, and a lane that ran ahead to the next load's address would change them
+// under the instruction still to be issued.
+__device__ __forceinline__ bool elect_one() {
   uint32_t lead;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "elect.sync _|p, 0xffffffff;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(lead));
-  return lead;
-}
-
-// umma_f16, umma_f16_ts and umma_commit of a whole warp, issued by the lane with lead != 0
-__device__ __forceinline__ void umma_f16_lead(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t accumulate, uint32_t lead) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "=r"(lead)
+      :
       : "memory");
-}
-__device__ __forceinline__ void umma_f16_ts_lead(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                                 uint32_t accumulate, uint32_t lead) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void umma_commit_lead(uint64_t* bar, uint32_t lead) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\t"
-      "setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-      "r"(lead)
-      : "memory");
+  return lead != 0;
 }
 
 // AB_FMT: 1 = bf16, 0 = f16; DP: 64 or 128, the head size of the tiles (64 <=
@@ -329,14 +307,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= kSoftmaxWarps) {  // producer, MMA
     bool ok = true, more = true;
-    if (warp == kWarpProducer) {
-      // -------------------------------------------------------------- producer (whole warp)
+    if (warp == kWarpK || warp == kWarpV) {
+      // -------------------------------------------------------------- producers (whole warps)
+      const int kv = warp == kWarpV;
+      const CUtensorMap* const map = kv ? &tmV : &tmK;
+      const uint8_t* const pool = kv ? p.v_pool : p.k_pool;
       if (lane == 0) {
-        tma_prefetch_desc(&tmQ);
-        tma_prefetch_desc(&tmK);
-        tma_prefetch_desc(&tmV);
+        if (kv == 0) tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(map);
       }
-      int buffer = 0, queries = 0;  // buffers and Q loads so far
+      int chunks = 0, queries = 0;  // chunks and Q loads so far
       // Lane l reads the page ids of tokens 4 l .. 4 l + 3 of a chunk, one chunk
       // ahead.  A chunk is page-granular if all tokens of every slab lie in the
       // page of the slab's first one.
@@ -363,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n_it = it.count();
         if (n_it == 0) continue;
         read_ids(it, it.chunk(0));
-        {
+        if (kv == 0) {
           bool got = true;
           if (lane == 0) {
             got = mbar_wait(q_empty, (queries & 1) ^ 1u, abort_flag);
@@ -379,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++queries;
           if (!__shfl_sync(0xffffffffu, got, 0)) break;
         }
-        for (int i = 0; i < n_it && ok; ++i) {
+        for (int i = 0; i < n_it && ok; ++i, ++chunks) {
           const int c = it.chunk(i);
           const int page = (int)resolve_page(id[0], p.num_pages);  // -1 where nothing was read
           bool gran = page >= 0;
@@ -390,38 +370,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int pg = __shfl_sync(0xffffffffu, page, (lane * per_slab) & 31);  // page of this lane's slab
           if (i + 1 < n_it) read_ids(it, it.chunk(i + 1));
           bool got = true;
-          int rows[4];
-          if (per_token) token_rows(p, it, c * kChunk, lane, rows);
-          for (int kv = 0; kv < 2; ++kv, ++buffer) {
-            const int buf = buffer % kNumBuf;
-            got = true;
-            if (lane == 0) {
-              got = mbar_wait(&buf_empty[buf], ((buffer / kNumBuf) & 1) ^ 1u, abort_flag);
-              if (got && !per_token) mbar_expect_tx(&buf_full[buf], kTileBytes);
-            }
-            if (!__shfl_sync(0xffffffffu, got, 0)) {
-              ok = false;
-              break;
-            }
+          const int buf = 2 * (chunks % (kNumBuf / 2)) + kv;
+          if (lane == 0) {
+            got = mbar_wait(&buf_empty[buf], ((chunks / (kNumBuf / 2)) & 1) ^ 1u, abort_flag);
+            if (got && !per_token) mbar_expect_tx(&buf_full[buf], kTileBytes);
+          }
+          if (!__shfl_sync(0xffffffffu, got, 0)) {
+            ok = false;
+            break;
+          }
+          __syncwarp();
+          uint8_t* dst = sBuf + buf * kTileBytes;
+          if (per_token) {
+            int rows[4];
+            token_rows(p, it, c * kChunk, lane, rows);
+            fill_tokens<DP>(dst, pool, rows, lane, p.D);
+            attn::cp_async_wait_all();  // each lane waits for its copies, fences them for the tensor cores
+            fence_proxy_async_smem();
             __syncwarp();
-            uint8_t* dst = sBuf + buf * kTileBytes;
-            if (per_token) {
-              fill_tokens<DP>(dst, kv ? p.v_pool : p.k_pool, rows, lane, p.D);
-              if (kv == 1) {  // each lane waits for its copies, fences them for the tensor cores, hands both over
-                attn::cp_async_wait_all();
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                  mbar_arrive(&buf_full[(buffer - 1) % kNumBuf]);
-                  mbar_arrive(&buf_full[buf]);
-                }
-              }
-            } else if (lane < ppc) {
-              const CUtensorMap* map = kv ? &tmV : &tmK;
-              const int row = ((pg * p.B + it.b) * p.Hkv + it.kvh) * p.ps + (c * kChunk + lane * p.slab) % p.ps;
+            if (lane == 0) mbar_arrive(&buf_full[buf]);
+          } else {
+            // one load after the other from a converged warp: coordinates and
+            // addresses in uniform registers, as for the products below
+            const int mine = ((pg * p.B + it.b) * p.Hkv + it.kvh) * p.ps + (c * kChunk + lane * p.slab) % p.ps;
+#pragma unroll 1
+            for (int u = 0; u < ppc; ++u) {
+              const int row = __shfl_sync(0xffffffffu, mine, u);
+              if (elect_one()) {
 #pragma unroll
-              for (int h = 0; h < kHalves; ++h)
-                tma_load_2d(dst + h * kHalfBytes + lane * p.slab * 128, map, h * 64, row, &buf_full[buf]);
+                for (int h = 0; h < kHalves; ++h)
+                  tma_load_2d(dst + h * kHalfBytes + u * p.slab * 128, map, h * 64, row, &buf_full[buf]);
+              }
+              __syncwarp();
             }
           }
         }
@@ -429,11 +409,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       attn::cp_async_wait_all();  // after an abort too: no copy of this warp may land after the block's end
     } else if (warp == kWarpMma) {
       // -------------------------------------------------------------- MMA issuer
-      // The whole warp walks the loop and one elected lane issues: with every
+      // The whole warp walks the loop and an elected lane issues: with every
       // value the same in all lanes, descriptors and addresses stay in uniform
       // registers (issued from a one-lane branch a product took ~90 cycles of
       // this warp, above the 64 it takes the tensor pipe).
-      const uint32_t lead = elect_one();
       const uint64_t q_desc = sw128_kmajor_desc(smem_u32(sQ));
       const uint64_t k_desc = sw128_kmajor_desc(smem_u32(sBuf));
       const uint64_t v_desc = sw128_mnmajor_desc(smem_u32(sBuf), kHalfBytes);
@@ -450,23 +429,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto issue_s = [&](int t, int k) {
         const uint32_t d = tmem_base + (uint32_t)(t * 128);
         const uint64_t qa = q_desc + (uint64_t)(t * (kTileBytes >> 4)), ka = k_desc + (uint64_t)(k * (kTileBytes >> 4));
+        if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < DP / 16; ++x) {
-          const uint32_t off = ((x >> 2) * kHalfBytes + (x & 3) * 32) >> 4;
-          umma_f16_lead(d, qa + off, ka + off, IDESC_S, x > 0, lead);
+          for (int x = 0; x < DP / 16; ++x) {
+            const uint32_t off = ((x >> 2) * kHalfBytes + (x & 3) * 32) >> 4;
+            umma_f16(d, qa + off, ka + off, IDESC_S, x > 0);
+          }
+          umma_commit(&s_full[t]);
         }
-        umma_commit_lead(&s_full[t], lead);
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit(bar);
+        __syncwarp();
       };
       // O_t += P_t V for the first 48 keys of each half of the chunk (part 0), or their last 16
       auto issue_pv = [&](int t, int k, int part, bool acc) {
         const uint32_t d = tmem_base + (uint32_t)(256 + t * 128);
         const uint32_t pa = tmem_base + (uint32_t)(t * 128);
         const uint64_t va = v_desc + (uint64_t)(k * (kTileBytes >> 4));
+        if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          if (((x & 3) == 3) == (part == 1))
-            umma_f16_ts_lead(d, pa + (x >> 2) * 64 + (x & 3) * 8, va + (uint64_t)((x * 16 * 128) >> 4), IDESC_PV, (acc || x > 0) ? 1u : 0u,
-                             lead);
+          for (int x = 0; x < 8; ++x)
+            if (((x & 3) == 3) == (part == 1))
+              umma_f16_ts(d, pa + (x >> 2) * 64 + (x & 3) * 8, va + (uint64_t)((x * 16 * 128) >> 4), IDESC_PV,
+                          (acc || x > 0) ? 1u : 0u);
+        }
+        __syncwarp();
       };
       for (int r = 0; ok; ++r) {
         const int index = item_index(p, r, &more);
@@ -481,8 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = wait(&buf_full[buf], phase))) break;
         if (n0 > 0) issue_s(0, buf);
         if (n1 > 0) issue_s(1, buf);
-        umma_commit_lead(&buf_empty[buf], lead);
-        if (n_it == 1) umma_commit_lead(q_empty, lead);
+        commit(&buf_empty[buf]);
+        if (n_it == 1) commit(q_empty);
 #pragma unroll 1
         for (int i = 0; i < n_it; ++i) {
           const int v = after(buf, 1), next = after(buf, 2);
@@ -499,16 +488,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(ok = wait(&p_full[2 * t + 1], p_phase[t]))) break;
               issue_pv(t, v, 1, true);
               p_phase[t] ^= 1u;
-              if (i + 1 == n_t) umma_commit_lead(&pv_done[t], lead);
-              if (t == 1 || i >= n1) umma_commit_lead(&buf_empty[v], lead);  // the last tile of the chunk
+              if (i + 1 == n_t) commit(&pv_done[t]);
+              if (t == 1 || i >= n1) commit(&buf_empty[v]);  // the last tile of the chunk
               if (i + 1 < n_t) {
                 if (t == 0 || i + 1 >= n0) {
                   if (!(ok = wait(&buf_full[next], next_phase))) break;
                 }
                 issue_s(t, next);
                 if (t == 1 || i + 1 >= n1) {
-                  umma_commit_lead(&buf_empty[next], lead);
-                  if (i + 2 == n_it) umma_commit_lead(q_empty, lead);
+                  commit(&buf_empty[next]);
+                  if (i + 2 == n_it) commit(q_empty);
                 }
               }
             }
@@ -518,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase = next_phase;
         }
       }
-      umma_commit_lead(drain, lead);
+      commit(drain);
       if (lane == 0) mbar_wait(drain, 0, abort_flag, /*honour_abort=*/false);
       __syncwarp();
     }
