@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         return got;
       };
       auto after = [&](int k, int n) { return k + n >= kNumBuf ? k + n - kNumBuf : k + n; };
-      auto issue_s = [&](int t, int k) {
+      // S of tile t; free: whether K's buffer and q: whether Q's are released behind it
+      auto issue_s = [&](int t, int k, bool free, bool q_free) {
         const uint32_t d = tmem_base + (uint32_t)(t * 128);
         const uint64_t qa = q_desc + (uint64_t)(t * (kTileBytes >> 4)), ka = k_desc + (uint64_t)(k * (kTileBytes >> 4));
         if (elect_one()) {
@@ -436,6 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_f16(d, qa + off, ka + off, IDESC_S, x > 0);
           }
           umma_commit(&s_full[t]);
+          if (free) umma_commit(&buf_empty[k]);
+          if (q_free) umma_commit(q_empty);
         }
         __syncwarp();
       };
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       };
       // O_t += P_t V for the first 48 keys of each half of the chunk (part 0), or their last 16
-      auto issue_pv = [&](int t, int k, int part, bool acc) {
+      auto issue_pv = [&](int t, int k, int part, bool acc, bool last, bool free) {
         const uint32_t d = tmem_base + (uint32_t)(256 + t * 128);
         const uint32_t pa = tmem_base + (uint32_t)(t * 128);
         const uint64_t va = v_desc + (uint64_t)(k * (kTileBytes >> 4));
@@ -454,6 +457,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (((x & 3) == 3) == (part == 1))
               umma_f16_ts(d, pa + (x >> 2) * 64 + (x & 3) * 8, va + (uint64_t)((x * 16 * 128) >> 4), IDESC_PV,
                           (acc || x > 0) ? 1u : 0u);
+          if (last) umma_commit(&pv_done[t]);
+          if (free) umma_commit(&buf_empty[k]);
         }
         __syncwarp();
       };
@@ -468,10 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = wait(q_full, q_phase))) break;
         q_phase ^= 1u;
         if (!(ok = wait(&buf_full[buf], phase))) break;
-        if (n0 > 0) issue_s(0, buf);
-        if (n1 > 0) issue_s(1, buf);
-        commit(&buf_empty[buf]);
-        if (n_it == 1) commit(q_empty);
+        if (n0 > 0) issue_s(0, buf, n1 == 0, n1 == 0 && n_it == 1);
+        if (n1 > 0) issue_s(1, buf, true, n_it == 1);
 #pragma unroll 1
         for (int i = 0; i < n_it; ++i) {
           const int v = after(buf, 1), next = after(buf, 2);
@@ -484,21 +487,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (t == 0 || i >= n0) {  // the first tile of the chunk
                 if (!(ok = wait(&buf_full[v], v_phase))) break;
               }
-              issue_pv(t, v, 0, i > 0);
+              issue_pv(t, v, 0, i > 0, false, false);
               if (!(ok = wait(&p_full[2 * t + 1], p_phase[t]))) break;
-              issue_pv(t, v, 1, true);
+              issue_pv(t, v, 1, true, i + 1 == n_t, t == 1 || i >= n1);  // V is free behind the chunk's last tile
               p_phase[t] ^= 1u;
-              if (i + 1 == n_t) commit(&pv_done[t]);
-              if (t == 1 || i >= n1) commit(&buf_empty[v]);  // the last tile of the chunk
               if (i + 1 < n_t) {
                 if (t == 0 || i + 1 >= n0) {
                   if (!(ok = wait(&buf_full[next], next_phase))) break;
                 }
-                issue_s(t, next);
-                if (t == 1 || i + 1 >= n1) {
-                  commit(&buf_empty[next]);
-                  if (i + 2 == n_it) commit(q_empty);
-                }
+                const bool last_tile = t == 1 || i + 1 >= n1;
+                issue_s(t, next, last_tile, last_tile && i + 2 == n_it);
               }
             }
           }
