@@ -91,12 +91,13 @@ WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
     const int64_t chunks = most / attn::kChunk + 1;
     // Fewer items than SMs, or a last round that leaves most of them idle: cut
     // the chunk lists.  Cost in chunks: a round is one piece and about 1.5
-    // chunks of set-up and output; joining the pieces costs about 3.
+    // chunks of set-up and output; joining the pieces costs a launch and writing
+    // and reading them (256 rows of D fp32 each; a chunk takes about 2 us).
     double best = 0;
     for (int n = 1; n <= 32 && n * 2 <= chunks + 1; ++n) {
       if (n > 1 && items * n > 8.0 * sms) break;
       const double rounds = (double)(int64_t)((items * n + sms - 1) / sms);
-      const double cost = rounds * ((double)chunks / n + 1.5) + (n > 1 ? 3.0 : 0.0);
+      const double cost = rounds * ((double)chunks / n + 1.5) + (n > 1 ? 2.0 + items * n * D * 1.6e-4 : 0.0);
       if (n == 1 || cost < best) {
         best = cost;
         p.splits = n;
@@ -219,7 +220,8 @@ int launch_split_inst(const split::Args& a, cudaStream_t s) {
   const unsigned grid = (unsigned)((a.max_warps + split::kWarps - 1) / split::kWarps);
   split::split_attention_kernel<T, DP, MANY><<<grid, split::kThreads, smem, s>>>(a);
   MTP_LAUNCH_CHECK();
-  const unsigned rows = (unsigned)((int64_t)a.B * a.row_tiles * a.Hkv * split::kRows);
+  const int64_t per_unit = (int64_t)a.S * a.G < split::kRows ? (int64_t)a.S * a.G : split::kRows;
+  const unsigned rows = (unsigned)((int64_t)a.B * a.row_tiles * a.Hkv * per_unit);
   return launch_dependent(split::split_merge_kernel<T>, rows, 1, split::kMergeWarps * 32, s, a);
 }
 

@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(Args a) {
   __shared__ int s_warp[kThreads / 32];
   __shared__ int s_digit, s_left;
   const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, tid = threadIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the moving kernel waits for this one's end
   const int len = length(a, b, h == 0 && tid == 0);
   const int n = min(len, a.budget);
   if (h == 0 && tid == 0) a.new_lens[b] = n;

@@ -287,6 +287,8 @@ __global__ void __launch_bounds__(kThreads) split_attention_kernel(Args a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * kWarps + warp;
   uint8_t* ring = smem + warp * (kStages * stage_bytes(DP));
+  // the joining kernel may be set up on SMs that run out of blocks; it waits for this one's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t ring_addr = smem_u32(ring);
 
   const Line line = find_block(a, [&](int64_t total) {
@@ -549,24 +551,19 @@ __global__ void __launch_bounds__(kMergeWarps * 32) split_merge_kernel(Args a) {
   __shared__ float s_m[kMergeWarps], s_l[kMergeWarps];
   __shared__ float s_o[kMergeWarps][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.x % kRows;
-  const int hk = (blockIdx.x / kRows) % a.Hkv;
-  const int pair = blockIdx.x / kRows / a.Hkv;
+  const int per_unit = min(kRows, a.S * a.G);  // rows of a tile that exist
+  const int r = blockIdx.x % per_unit;
+  const int hk = (blockIdx.x / per_unit) % a.Hkv;
+  const int pair = blockIdx.x / per_unit / a.Hkv;
   const int b = pair / a.row_tiles, row = (pair % a.row_tiles) * kRows + r;
   if (row >= a.S * a.G) return;
   const Tile t = tile_of(a, pair);
   const int D = a.D;
   const int64_t head = ((int64_t)b * a.S + row / a.G) * a.Hq + (int64_t)hk * a.G + row % a.G;
   T* dst = static_cast<T*>(a.out) + head * D;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (r >= t.rows) {
-    for (int d = threadIdx.x; d < D; d += blockDim.x) dst[d] = rowattn::from_f32<T>(0.f);
-    if (a.scores && threadIdx.x == 0) a.row_ml[head * 2] = a.row_ml[head * 2 + 1] = 0.f;
-    return;
-  }
+  // all that needs no piece is worked out while the pieces are still being made
   const int nblk = blocks_of(t);
-  // blocks of the line before this pair, and in all
-  int64_t before = 0, total = 0;
+  int64_t before = 0, total = 0;  // blocks of the line before this pair, and in all
   for (int p = lane; p < a.B * a.row_tiles; p += 32) {
     const int64_t n = (int64_t)blocks_of(tile_of(a, p)) * a.Hkv;
     total += n;
@@ -579,6 +576,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) split_merge_kernel(Args a) {
   }
   const int64_t first = before + (int64_t)hk * nblk;
   const int64_t used = warps_used(total, a.max_warps, a.min_blocks);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (r >= t.rows) {
+    for (int d = threadIdx.x; d < D; d += blockDim.x) dst[d] = rowattn::from_f32<T>(0.f);
+    if (a.scores && threadIdx.x == 0) a.row_ml[head * 2] = a.row_ml[head * 2 + 1] = 0.f;
+    return;
+  }
   const int64_t w0 = piece_owner(total, used, first), w1 = piece_owner(total, used, first + nblk - 1);
   if (w0 == w1) return;  // one warp had it all and wrote it
   auto slot_of = [&](int64_t w) {
