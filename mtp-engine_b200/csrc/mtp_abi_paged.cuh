@@ -198,7 +198,6 @@ int launch_prompt(const split::Args& a, const WindowPlan& pl, cudaStream_t s) {
   p.splits = pl.splits;
   p.items = a.B * a.Hkv * pl.pairs * pl.splits;
   p.table_vec = aligned16(a.page_table) && a.table_stride % 4 == 0;
-  p.dtype = a.dtype;
   p.scale_log2 = a.scale_log2;
   int dev;
   if (int st = current_device(&dev)) return st;
@@ -412,7 +411,6 @@ int mtp_paged_window_attention(const mtp_paged_window_attention_args* args) {
   a.dtype = dtype;
   a.window = window == 0 || window > kNoWindow ? kNoWindow : (int)window;
   a.sinks = window == 0 ? 0 : (int)(sinks < kNoWindow ? sinks : kNoWindow);
-  a.scale = scale;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.row_tiles = p.row_tiles;
   a.max_warps = p.max_warps;

@@ -73,7 +73,6 @@ struct Params {
   int splits;    // pieces of a pair's chunk list
   int items;     // B * Hkv * pairs * splits
   int table_vec; // page-table rows 16-byte aligned
-  int dtype;
   float scale_log2;
 };
 

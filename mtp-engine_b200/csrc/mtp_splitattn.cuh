@@ -56,7 +56,7 @@ struct Args {
   int B, S, Hq, Hkv, G, D, dtype;
   int window;  // 2^30: everything
   int sinks;
-  float scale, scale_log2;
+  float scale_log2;  // softmax scale * log2(e)
   int row_tiles;    // ceil(S * G / kRows)
   int max_warps;    // warps of the launch
   int min_blocks;   // least blocks a warp takes

@@ -608,6 +608,58 @@ def test_side_stream(mk):
     assert torch.equal(out, want)
 
 
+def test_offsets_past_32_bits(mk):
+    """Pools of more than 2^31 elements: pages behind that mark give the same
+    bits as the same pages in a small pool."""
+    B, Hq, Hkv, D, ps, S, n = 1, 4, 1, 128, 16, 40, 300
+    dt = torch.bfloat16
+    used = -(-n // ps)
+    big = (1 << 31) // (ps * D) + used + 8
+    if torch.cuda.mem_get_info()[0] < 3 * big * ps * D * 2:
+        pytest.skip("not enough memory")
+    g = torch.Generator().manual_seed(6)
+    small = [dev(x) for x in pools(g, used, B, Hkv, ps, D, dt)]
+    order = torch.randperm(used, generator=g)
+    small_table = order[torch.arange(n) // ps][None].to(torch.int32)
+    huge = [torch.empty(big, B, Hkv, ps, D, dtype=dt, device="cuda") for _ in range(2)]
+    for a, b in zip(huge, small):
+        a[big - used:] = b
+    x = dev(randn(g, B, S, Hq + 2 * Hkv, D, dtype=dt))
+    cos, sin = (dev(t) for t in angles(n, D))
+    lens, new = torch.tensor([n]).cuda(), torch.tensor([S]).cuda()
+    results = []
+    for (kp, vp), table in ((small, dev(small_table)), (huge, dev(small_table + (big - used)))):
+        w = torch.linspace(0, 1, n).view(1, 1, n).cuda().contiguous()
+        q = mk.fused_qk_norm_rope_paged(x[:, :, :Hq], x[:, :, Hq:Hq + Hkv], x[:, :, Hq + Hkv:], None, cos, sin, kp, vp,
+                                        table, lens - S)
+        a = mk.fused_paged_prompt_attention(q, kp, vp, table, lens, new)
+        d = mk.fused_paged_decode_attention(q[:, -1], kp, vp, table, lens, key_weights=w)
+        kept, _ = mk.paged_kv_evict(kp, vp, table, lens, w, 100, sinks=3, recent=10)
+        results.append((q, a, d, w, kept, kp[-used:], vp[-used:]))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_rows_of_a_batch_do_not_depend_on_it(mk):
+    """A sequence gives the same bits of queries and caches alone and in a
+    padded batch, and the same attention up to the joins' order."""
+    g = torch.Generator().manual_seed(9)
+    B, S, Hq, Hkv, D, ps = 3, 150, 8, 2, 128, 16
+    lens, new = [150, 400, 9], [150, 30, 9]
+    L = 400
+    P = L // ps
+    table = R.make_table(B, L, P, ps, 5)
+    kp, vp = (dev(x) for x in pools(g, P, B, Hkv, ps, D, torch.bfloat16))
+    q = dev(randn(g, B, S, Hq, D, dtype=torch.bfloat16))
+    out = mk.fused_paged_prompt_attention(q, kp, vp, dev(table), torch.tensor(lens).cuda(), torch.tensor(new).cuda())
+    for b in range(B):
+        one = mk.fused_paged_prompt_attention(q[b:b + 1, :new[b]], kp[:, b:b + 1], vp[:, b:b + 1], dev(table[b:b + 1]),
+                                              torch.tensor(lens[b:b + 1]).cuda())
+        # either is within half a step of the output and half a step of every weight; |v| < 6
+        assert (one[0].double() - out[b, :new[b]].double()).abs().max() <= 4 * 2.0 ** -8 * 6
+        assert not out[b, new[b]:].any()
+
+
 def test_empty_calls(mk):
     z = torch.zeros
     kp = z(2, 0, 1, 16, 64, dtype=torch.bfloat16).cuda()
