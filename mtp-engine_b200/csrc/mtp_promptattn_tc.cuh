@@ -33,7 +33,11 @@
 //
 // Bound: the two products of a chunk take 2 x 512 tensor cycles per tile
 // (D = 128) and its 16384 exponentials 1024 cycles of the SM's exp2 units, so
-// 2048 cycles per chunk for both tiles is the floor of either pipe.
+// 2048 cycles per chunk for both tiles is the floor of either pipe.  Measured
+// (B200, Hq 32, Hkv 8, D 128, bf16, 16-token pages): one causal prompt of 8192
+// tokens 532 us (1034 TFLOP/s, ~3650 cycles per chunk), 594 us in calls back to
+// back under the power cap; two prompts of 2750 and 5501 tokens with a window of
+// 1024 216 us; 512 tokens behind 32000 354 us, 26 of them the joining of pieces.
 #pragma once
 
 #include "mtp_attention_tc.cuh"
