@@ -180,6 +180,10 @@ PROMPT = [
     (1, 30, 3, 1, 20, 16, [20], [30], None, 0, torch.float16, False),
     (1, 20, 16, 1, 128, 16, [1500], [20], None, 0, torch.bfloat16, False),  # few rows, a long cache
     (1, 9, 130, 1, 64, 16, [40], [9], None, 0, torch.bfloat16, False),  # more heads than a tile has rows
+    (1, 20, 2, 2, 128, 16, [3], [20], None, 0, torch.bfloat16, False),  # fewer positions than a tile has
+    (2, 17, 1, 1, 64, 3, [0, 2], [17, 5], None, 0, torch.float16, False),  # pages of three tokens
+    (2, 600, 2, 1, 96, 64, [0, 200], [333, 600], 130, 2, torch.bfloat16, False),  # several items, a short window
+    (1, 300, 8, 1, 64, 16, [900], [300], 256, 300, torch.float16, True),  # sinks over whole chunks, scattered tokens
 ]
 
 
@@ -660,6 +664,33 @@ def test_rows_of_a_batch_do_not_depend_on_it(mk):
         assert not out[b, new[b]:].any()
 
 
+def test_two_streams_at_once(mk):
+    """Calls that overlap on two streams do not meet in scratch memory."""
+    g = torch.Generator().manual_seed(3)
+    B, Hq, Hkv, D, ps, n = 1, 8, 2, 128, 16, 3000
+    P = -(-n // ps)
+    table, lens = dev(R.make_table(B, n, P, ps, 5)), torch.tensor([n]).cuda()
+    data = []
+    for _ in range(2):
+        kp, vp = (dev(x) for x in pools(g, P, B, Hkv, ps, D, torch.bfloat16))
+        data.append((dev(randn(g, B, Hq, D, dtype=torch.bfloat16)), dev(randn(g, B, 50, Hq, D, dtype=torch.bfloat16)),
+                     kp, vp))
+    call = lambda q, p, kp, vp: (mk.fused_paged_decode_attention(q, kp, vp, table, lens),
+                                 mk.fused_paged_prompt_attention(p, kp, vp, table, lens))
+    want = [call(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(*data[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for pair in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(pair, want[i]))
+
+
 def test_empty_calls(mk):
     z = torch.zeros
     kp = z(2, 0, 1, 16, 64, dtype=torch.bfloat16).cuda()
@@ -673,6 +704,8 @@ def test_empty_calls(mk):
     t0, l0 = z(1, 0, dtype=torch.int32).cuda(), z(1, dtype=torch.int32).cuda()
     out = mk.fused_paged_decode_attention(torch.ones(1, 2, 64, dtype=torch.bfloat16).cuda(), kp, kp, t0, l0)
     assert not out.any()
+    out = mk.fused_paged_prompt_attention(torch.ones(1, 40, 2, 64, dtype=torch.bfloat16).cuda(), kp, kp, t0, l0, l0)
+    assert out.shape == (1, 40, 2, 64) and not out.any()
     cos, sin = (dev(t) for t in angles(4, 64))
     q, k = mk.fused_qk_norm_rope(z(1, 0, 2, 64).cuda(), z(1, 0, 1, 64).cuda(), z(1, 0, dtype=torch.int32).cuda(), cos,
                                  sin)
