@@ -60,6 +60,7 @@ struct WindowPlan {
   int dp = 0;  // head size of the tiles
   int row_tiles = 1, max_warps = 1, min_blocks = 1;
   int tpt = 0, pairs = 0, splits = 1;  // tensor-core tiles
+  int window = kNoWindow, sinks = 0;   // as the kernels take them
   int64_t score_ld = 0;
   size_t part_o = 0, part_ml = 0, scores = 0, row_ml = 0;  // bytes
   size_t total() const { return part_o + part_ml + scores + row_ml + 256; }
@@ -75,6 +76,14 @@ constexpr int kSplitMinBlocks = 4;
 WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_keys, int64_t window,
                        int64_t sinks, int dtype, bool aligned, bool weights) {
   WindowPlan p;
+  // The caller's window and sinks may be anything up to 2^63 - 1 ("everything").
+  // Brought below 2^30 here, before any sum with them: the sizes below and the
+  // kernels go by the same values.
+  if (window > 0 && window <= kNoWindow) {
+    p.window = (int)window;
+    p.sinks = (int)(sinks < 0 ? 0 : (sinks < kNoWindow ? sinks : kNoWindow));
+  }
+  const int64_t reach = (int64_t)p.window + p.sinks;  // the most keys that one row sees
   const int64_t G = Hq / Hkv;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -87,7 +96,7 @@ WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
     p.pairs = (int)((S + 2 * p.tpt - 1) / (2 * p.tpt));
     const double items = (double)B * Hkv * p.pairs;
     int64_t most = max_keys;
-    if (window > 0 && window + sinks + 2 * p.tpt < most) most = window + sinks + 2 * p.tpt;
+    if (reach + 2 * p.tpt < most) most = reach + 2 * p.tpt;
     const int64_t chunks = most / attn::kChunk + 1;
     // Fewer items than SMs, or a last round that leaves most of them idle: cut
     // the chunk lists.  Cost in chunks: a round is one piece and about 1.5
@@ -112,7 +121,7 @@ WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
   }
   if (wide) {
     int64_t most = max_keys;  // keys that one tile of rows sees
-    if (window > 0 && window + sinks + split::kRows < most) most = window + sinks + split::kRows;
+    if (reach + split::kRows < most) most = reach + split::kRows;
     p.path = kPathSplit;
     p.dp = D <= 64 ? 64 : (D <= 128 ? 128 : 256);
     p.row_tiles = (int)((S * G + split::kRows - 1) / split::kRows);
@@ -127,8 +136,7 @@ WindowPlan window_plan(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
   }
   if (weights) {
     p.score_ld = (max_keys + split::kKeys - 1) / split::kKeys * split::kKeys;
-    if (window > 0 && window + sinks + split::kKeys < p.score_ld)
-      p.score_ld = (window + sinks + split::kKeys) / split::kKeys * split::kKeys;
+    if (reach + split::kKeys < p.score_ld) p.score_ld = (reach + split::kKeys) / split::kKeys * split::kKeys;
     p.scores = align256((size_t)B * Hq * p.score_ld * 4);
     p.row_ml = align256((size_t)B * Hq * 2 * 4);
   }
@@ -409,8 +417,8 @@ int mtp_paged_window_attention(const mtp_paged_window_attention_args* args) {
   a.G = (int)(Hq / Hkv);
   a.D = (int)D;
   a.dtype = dtype;
-  a.window = window == 0 || window > kNoWindow ? kNoWindow : (int)window;
-  a.sinks = window == 0 ? 0 : (int)(sinks < kNoWindow ? sinks : kNoWindow);
+  a.window = p.window;
+  a.sinks = p.sinks;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.row_tiles = p.row_tiles;
   a.max_warps = p.max_warps;
