@@ -24,6 +24,7 @@
 //               0 * NaN is NaN).  Two warps because a page load takes one of
 //               them 100 cycles and more, 32 loads a chunk with 16-token pages
 //   warp 17     tcgen05.mma issuer
+//   warp 19     of the first block: records lengths outside their range, once per launch
 // All rings and barrier phases run on from item to item: the next item's keys
 // are already on their way, and its first scores are computed, while the
 // softmax warps write the last item's output.
@@ -49,7 +50,7 @@ namespace prompt {
 using attn::kChunk;
 constexpr int kThreads = 640;  // 96 registers each
 constexpr int kSoftmaxWarps = 16;
-constexpr int kWarpK = 16, kWarpMma = 17, kWarpV = 18;
+constexpr int kWarpK = 16, kWarpMma = 17, kWarpV = 18, kWarpCheck = 19;
 constexpr int kHalfBytes = 128 * 128;  // 128 rows x 64 dims
 constexpr int tile_bytes(int dp) { return dp / 64 * kHalfBytes; }
 constexpr int num_buf(int dp) { return dp == 128 ? 4 : 8; }  // 128 KB of K and V in flight
@@ -109,10 +110,9 @@ __device__ __forceinline__ Item item_of(const Params& p, int index) {
   u /= p.Hkv;
   it.b = u % p.B;
   it.s0 = (p.pairs - 1 - u / p.B) * 2 * p.tpt;  // the last positions first
-  const int cap = (int)min(p.table_stride, (int64_t)INT32_MAX);
-  it.len = max(0, min(__ldg(p.seq_lens + it.b), cap));
-  const int n = p.q_lens ? __ldg(p.q_lens + it.b) : p.S;
-  it.n = max(0, min(n, min(p.S, it.len)));
+  const split::Seq seq = split::lengths(p.seq_lens, p.q_lens, p.table_stride, p.S, it.b);
+  it.len = seq.len;
+  it.n = seq.n;
   it.ns = it.c_lo = it.i0 = it.n_it[0] = it.n_it[1] = 0;
   it.call_lo = max(0, it.len - it.n - p.window + 1);
   if (it.s0 >= it.n) return it;
@@ -511,6 +511,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit(drain);
       if (lane == 0) mbar_wait(drain, 0, abort_flag, /*honour_abort=*/false);
       __syncwarp();
+    } else if (warp == kWarpCheck && blockIdx.x == 0) {
+      for (int b = lane; b < p.B; b += 32) split::lengths(p.seq_lens, p.q_lens, p.table_stride, p.S, b, true);
     }
   } else {
     // ---------------------------------------------------------------- softmax
@@ -721,9 +723,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(Params p) {
   const int kvh = h / p.G, g = h % p.G;
   const int pair = s / (2 * p.tpt), t = s / p.tpt % 2, r = (s % p.tpt) * p.G + g;
   const int64_t base = (((int64_t)(p.pairs - 1 - pair) * p.B + b) * p.Hkv + kvh) * p.splits;
-  const int cap = (int)min(p.table_stride, (int64_t)INT32_MAX);
-  const int len = max(0, min(p.seq_lens[b], cap));
-  const int n = max(0, min(p.q_lens ? p.q_lens[b] : p.S, min(p.S, len)));
+  const int n = split::lengths(p.seq_lens, p.q_lens, p.table_stride, p.S, b).n;
   T* out = static_cast<T*>(p.out) + row * p.D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;

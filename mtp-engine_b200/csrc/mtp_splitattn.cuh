@@ -81,15 +81,20 @@ struct Seq {
 
 // Lengths as the caller's device arrays give them, forced into range (an entry
 // outside it is recorded once, by the caller that passes report).
-__device__ __forceinline__ Seq sequence(const Args& a, int b, bool report = false) {
-  const int len = a.seq_lens[b];
-  const int cap = (int)min(a.table_stride, (int64_t)INT32_MAX);
+__device__ __forceinline__ Seq lengths(const int32_t* seq_lens, const int32_t* q_lens, int64_t table_stride, int S,
+                                       int b, bool report = false) {
+  const int len = __ldg(seq_lens + b);
+  const int cap = (int)min(table_stride, (int64_t)INT32_MAX);
   Seq s;
   s.len = max(0, min(len, cap));
-  const int n = a.q_lens ? a.q_lens[b] : min(a.S, s.len);
-  s.n = max(0, min(n, min(a.S, s.len)));
+  const int n = q_lens ? __ldg(q_lens + b) : min(S, s.len);
+  s.n = max(0, min(n, min(S, s.len)));
   if (report && (s.len != len || s.n != n)) record_error(MTP_ERR_DEVICE);
   return s;
+}
+
+__device__ __forceinline__ Seq sequence(const Args& a, int b, bool report = false) {
+  return lengths(a.seq_lens, a.q_lens, a.table_stride, a.S, b, report);
 }
 
 // Visible keys of rows s0 .. s1 of a sequence: numbers [0, sinks) are the keys

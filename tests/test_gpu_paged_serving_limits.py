@@ -43,3 +43,45 @@ def test_far_windows_are_no_window(mk, dtype, D):
     out, got, _ = calls(window=5, sinks=sys.maxsize)
     within(out, ref[:, 0], tol[:, 0])
     within(got, w, wtol + w * 2.0 ** -23)
+
+
+# --------------------------------------------------------------------------- #
+# lengths outside their range
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("S,Hq,D,dtype,width", [
+    (5, 2, 64, torch.bfloat16, 40),     # 16-row tiles
+    (40, 2, 64, torch.bfloat16, 40),    # 128-row tiles
+    (40, 4, 128, torch.float16, 3000),  # pieces of the key axis, joined
+    (40, 2, 64, torch.float32, 40),     # row by row
+])
+def test_bad_lengths_are_recorded_on_every_path(mk, S, Hq, D, dtype, width):
+    """Lengths are forced into [0, table width] and [0, min(S, length)], and
+    recorded whichever kernel serves the call."""
+    g = torch.Generator().manual_seed(4)
+    B, ps = 40, 16  # more sequences than lanes; the bad ones lie behind the first 32
+    P = -(-width // ps)
+    kp, vp = (dev(t) for t in pools(g, P, B, 1, ps, D, dtype))
+    table = dev(R.make_table(B, width, P, ps, 3))
+    q = dev(randn(g, B, S, Hq, D, dtype=dtype))
+
+    def call(lens, new=None):
+        t = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32).cuda()
+        out = mk.fused_paged_prompt_attention(q, kp, vp, table, t(lens), t(new))
+        return out, status()
+
+    ok = [min(width, 7 * b) for b in range(B)]
+    good, code = call(ok)  # a sequence shorter than S has that many rows: in range
+    assert code == 0
+    for b, bad, forced in ((35, width + 1, width), (38, -2, 0), (39, 2 ** 31 - 1, width)):
+        want, code = call(ok[:b] + [forced] + ok[b + 1:])
+        assert code == 0
+        got, code = call(ok[:b] + [bad] + ok[b + 1:])
+        assert code == 7 and torch.equal(got, want), b
+    new = [min(S, n) for n in ok]
+    out, code = call(ok, new)
+    assert code == 0 and torch.equal(out, good)
+    for b, bad, forced in ((1, 8, min(S, 7)), (34, S + 1, S), (37, -1, 0), (39, -2 ** 31, 0)):
+        want, code = call(ok, new[:b] + [forced] + new[b + 1:])
+        assert code == 0
+        got, code = call(ok, new[:b] + [bad] + new[b + 1:])
+        assert code == 7 and torch.equal(got, want), b
