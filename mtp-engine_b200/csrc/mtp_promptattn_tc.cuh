@@ -211,6 +211,9 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
   }
 }
 
+// In place of an exchanged value: a signalling NaN, which no arithmetic gives.
+constexpr uint32_t kGone = 0x7fa5a5a5u;
+
 // P of 16 scores: 2^(s * mul - m) packed as 16-bit pairs, with the running sums
 // in (ls0, ls1).
 template <int AB_FMT>
@@ -524,7 +527,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem_base + lane_off + (uint32_t)(t * 128 + half * 64);  // this half's scores
     const uint32_t p_addr = s_addr;  // and its P, over the first 32 of its 64 columns
     const uint32_t o_addr = tmem_base + lane_off + (uint32_t)(256 + t * 128 + half * (DP / 2));  // half of the output
-    // the two warps that share 32 rows tell each other a value per row
+    // The two warps that share 32 rows tell each other a value per row.  They
+    // meet at a named barrier, which knows no limit, so they go through the same
+    // number of exchanges whatever their waits come to: a warp whose wait ran
+    // out still meets its partner once, with kGone in place of a value, and both
+    // leave behind that exchange.
     float* const ex_mine = sExchange + (t * 2 + half) * 128 + row;
     float* const ex_other = sExchange + (t * 2 + (half ^ 1)) * 128 + row;
     int turn = 0;
@@ -552,6 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < n_it; ++i) {
         const int first = it.chunk(i) * kChunk + half * 64;
         if (!__all_sync(0xffffffffu, wait_bar(&s_full[t], (done + i) & 1, abort_flag))) {
+          exchange(__uint_as_float(kGone));
           ok = false;
           break;
         }
@@ -578,8 +586,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k)
             m4[k] = attn::fmax3(m4[k], __uint_as_float(sc[k][j]), __uint_as_float(sc[k][j + 1]));
         const float mx = p.scale_log2 * fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float other = exchange(mx);
+        if (__any_sync(0xffffffffu, __float_as_uint(other) == kGone)) {
+          ok = false;
+          break;
+        }
         // both halves go by the greater maximum
-        const float m_new = attn::fmax3(m_run, mx, exchange(mx));
+        const float m_new = attn::fmax3(m_run, mx, other);
         if (i > 0) {
           // The scores of this chunk were issued after the last chunk's P V, so
           // O and P's columns are free here without another wait.
@@ -642,9 +655,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       done += n_it;
       if (n_it > 0) {
         l_run += exchange(l_run);
-        if (!__all_sync(0xffffffffu, wait_bar(&pv_done[t], finished & 1, abort_flag))) break;
+        const bool got = __all_sync(0xffffffffu, wait_bar(&pv_done[t], finished & 1, abort_flag));
         ++finished;
         tc_fence_after();
+        if (!got) continue;  // no output; on to the next item's first exchange
       }
       constexpr int kCols = DP / 2;  // this half's columns of the output
       const int col0 = half * kCols;
