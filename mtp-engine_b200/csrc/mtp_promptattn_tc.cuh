@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                               it.b, q_full);
             }
           }
-          ++queries;
           if (!__shfl_sync(0xffffffffu, got, 0)) break;
+          ++queries;
         }
         for (int i = 0; i < n_it && ok; ++i, ++chunks) {
           const int c = it.chunk(i);
@@ -412,7 +412,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      attn::cp_async_wait_all();  // after an abort too: no copy of this warp may land after the block's end
+      // After an abort too: no copy of this warp may land after the block's end.
+      // Page loads whose chunk nobody waits for any more are among the last
+      // kNumBuf / 2; each wait has its own limit and goes on although others gave up.
+      attn::cp_async_wait_all();
+      if (lane == 0) {
+        constexpr int kRing = kNumBuf / 2;
+        for (int j = max(0, chunks - kRing); j < chunks; ++j)
+          mbar_wait(&buf_full[2 * (j % kRing) + kv], (j / kRing) & 1, abort_flag, /*honour_abort=*/false);
+        if (queries > 0) mbar_wait(q_full, (queries - 1) & 1, abort_flag, /*honour_abort=*/false);
+      }
+      __syncwarp();
     } else if (warp == kWarpMma) {
       // -------------------------------------------------------------- MMA issuer
       // The whole warp walks the loop and an elected lane issues: with every

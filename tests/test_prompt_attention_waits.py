@@ -120,3 +120,29 @@ def test_the_kernel_has_that_form():
     assert sorted(re.findall(r"(?:if \([^\n]*\) )?break;", loop)) == \
         ["break;", "break;", "if (!more) break;", "if (!ok) break;"]
     assert "return" not in loop[:loop.index("tc_fence_before();\n  __syncthreads();")]
+
+
+def test_loads_land_before_the_block_ends():
+    """After a wait ran out, page loads may still be under way into shared
+    memory that the SM's next block will own: each producer waits (with a
+    limit) for the loads it has issued, a full ring of chunks and the queries.
+    `chunks` and `queries` count issued loads only."""
+    src = open(os.path.join(REPO, "mtp-engine_b200", "csrc", "mtp_promptattn_tc.cuh")).read()
+    code = re.sub(r"//[^\n]*|/\*.*?\*/ *", "", src)
+    role = code[code.index("if (warp == kWarpK || warp == kWarpV)"):code.index("} else if (warp == kWarpMma) {")]
+    tail = role[role.index("attn::cp_async_wait_all();\n      if (lane == 0)"):]
+    assert re.search(r"for \(int j = max\(0, chunks - kRing\); j < chunks; \+\+j\)\s*"
+                     r"mbar_wait\(&buf_full\[2 \* \(j % kRing\) \+ kv\], \(j / kRing\) & 1, abort_flag, false\);", tail)
+    assert re.search(r"if \(queries > 0\) mbar_wait\(q_full, \(queries - 1\) & 1, abort_flag, false\);", tail)
+    # counted behind the wait that may give up
+    assert re.search(r"if \(!__shfl_sync\(0xffffffffu, got, 0\)\) break;\s*\+\+queries;", role)
+    assert role.count("++queries") == 1 and role.count("++chunks") == 1
+    assert re.search(r"for \(int i = 0; i < n_it && ok; \+\+i, \+\+chunks\)", role)
+    # the fills of one buffer: chunk j is fill j / ring, and nothing is filled again behind the last ring
+    for ring in (2, 4):
+        for chunks in range(12):
+            last = {}
+            for j in range(chunks):
+                last[j % ring] = j // ring
+            waited = {j % ring: j // ring for j in range(max(0, chunks - ring), chunks)}
+            assert waited == last
