@@ -718,8 +718,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (row_ok && half == 0) {
-          p.part_ml[slot * 2] = m_run;  // -inf: no key of this piece is visible, and its output is not read
-          p.part_ml[slot * 2 + 1] = l_run;
+          p.part_ml[slot * 2] = m_run;
+          p.part_ml[slot * 2 + 1] = l_run;  // 0: no key of this piece is visible, and its output is not read
         }
       }
       // the next item's products overwrite O only after this warp's next arrival at p_full
@@ -758,10 +758,11 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(Params p) {
 #pragma unroll 4
     for (int i = 0; i < p.splits; ++i) {
       const int64_t slot = (base + i) * 256 + t * 128 + r;
-      const float m = p.part_ml[slot * 2];
-      if (m == -INFINITY) continue;
-      const float w = attn::ex2(m - M);
-      L += w * p.part_ml[slot * 2 + 1];
+      const float m = p.part_ml[slot * 2], l = p.part_ml[slot * 2 + 1];
+      if (l == 0.f) continue;  // no key of this piece is visible to the row: its output may not be written
+      // -inf with a sum is a NaN query's (a maximum passes NaN over, the sum holds it): 0 * NaN stays NaN
+      const float w = m == -INFINITY ? 0.f : attn::ex2(m - M);
+      L += w * l;
       if (mine) {
         const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot * p.D + lane * 4);
         acc[0] += w * v.x;

@@ -634,16 +634,22 @@ __global__ void __launch_bounds__(kMergeWarps * 32) split_merge_kernel(Args a) {
     for (int i = 0; i < 4; ++i)
       if ((h * 32 + lane) * 4 < D) s_o[warp][(h * 32 + lane) * 4 + i] = acc[h][i];
   __syncthreads();
-  float M = -INFINITY, L = 0.f;
+  // A maximum of -inf comes with nothing (a warp that had no piece: sums of 0)
+  // or with NaN scores (a maximum passes them over, the sums hold them): the
+  // sums are multiplied by 0, not left out, so that a NaN query stays NaN.
+  float M = -INFINITY, L = 0.f, f[kMergeWarps];
 #pragma unroll
   for (int i = 0; i < kMergeWarps; ++i) M = fmaxf(M, s_m[i]);
 #pragma unroll
-  for (int i = 0; i < kMergeWarps; ++i) L += s_m[i] == -INFINITY ? 0.f : s_l[i] * exp2_fast(s_m[i] - M);
+  for (int i = 0; i < kMergeWarps; ++i) {
+    f[i] = s_m[i] == -INFINITY ? 0.f : exp2_fast(s_m[i] - M);
+    L += s_l[i] * f[i];
+  }
   const float inv = L > 0.f ? 1.0f / L : 0.f;
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < kMergeWarps; ++i) v += s_m[i] == -INFINITY ? 0.f : s_o[i][d] * exp2_fast(s_m[i] - M);
+    for (int i = 0; i < kMergeWarps; ++i) v += s_o[i][d] * f[i];
     dst[d] = rowattn::from_f32<T>(v * inv);
   }
   if (a.scores && threadIdx.x == 0) {

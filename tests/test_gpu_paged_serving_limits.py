@@ -85,3 +85,46 @@ def test_bad_lengths_are_recorded_on_every_path(mk, S, Hq, D, dtype, width):
         assert code == 0
         got, code = call(ok, new[:b] + [bad] + new[b + 1:])
         assert code == 7 and torch.equal(got, want), b
+
+
+# --------------------------------------------------------------------------- #
+# NaN queries
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("S,Hq,D,dtype,n", [
+    (1, 4, 128, torch.bfloat16, 60), (1, 4, 128, torch.bfloat16, 5000), (1, 20, 64, torch.float16, 3000),
+    (4, 4, 128, torch.float16, 4000), (40, 4, 128, torch.bfloat16, 60), (40, 4, 128, torch.bfloat16, 5000),
+    (70, 7, 80, torch.float16, 3000), (1, 2, 40, torch.float32, 500), (3, 2, 40, torch.float32, 500),
+])
+def test_nan_queries_stay_nan(mk, S, Hq, D, dtype, n):
+    """A NaN in a query makes that row NaN, in one piece or in joined pieces,
+    and leaves every other row's bits alone."""
+    g = torch.Generator().manual_seed(4)
+    B, ps = 2, 16
+    P = -(-n // ps)
+    kp, vp = (dev(t) for t in pools(g, P, B, 1, ps, D, dtype))
+    table = dev(R.make_table(B, n, P, ps, 3))
+    q = dev(randn(g, B, S, Hq, D, dtype=dtype))
+    lens = torch.tensor([n, n // 2]).cuda()
+
+    def call(x):
+        out = [mk.fused_paged_prompt_attention(x, kp, vp, table, lens)]
+        if S == 1:
+            out.append(mk.fused_paged_decode_attention(x[:, 0], kp, vp, table, lens)[:, None])
+        return out
+
+    bad = q.clone()
+    hit = torch.zeros(B, S, Hq, dtype=torch.bool)
+    for b, s, h in ((0, S - 1, 1), (1, 0, Hq - 1), (1, S // 2, 0)):
+        bad[b, s, h, 3] = float("nan")
+        hit[b, s, h] = True
+    for good, got in zip(call(q), call(bad)):
+        assert torch.isfinite(good).all()
+        assert got.cpu()[hit].isnan().all()
+        assert torch.equal(got.cpu()[~hit], good.cpu()[~hit])
+    if S > 1:
+        return
+    w = [torch.zeros(B, 1, n, device="cuda") for _ in range(2)]
+    bad[1] = q[1]
+    for x, t in zip((q, bad), w):
+        mk.fused_paged_decode_attention(x[:, 0], kp, vp, table, lens, key_weights=t)
+    assert w[1][0, 0].isnan().all() and torch.equal(w[0][1], w[1][1])  # that key head's totals alone
