@@ -275,15 +275,16 @@ int mtp_qk_norm_rope(const mtp_qk_norm_rope_args* args) {
   if ((q_weight && (!valid_dtype(q_weight_dtype) || q_weight_dtype == MTP_DTYPE_E4M3)) ||
       (k_weight && (!valid_dtype(k_weight_dtype) || k_weight_dtype == MTP_DTYPE_E4M3)))
     return fail(MTP_ERR_DTYPE, "unsupported norm weight dtypes %d, %d", q_weight_dtype, k_weight_dtype);
+  // sizes before any sum or product of them, which would wrap
+  if (B > INT32_MAX / 2 || S > INT32_MAX / 2 || Hq > INT32_MAX / 2 || Hkv > INT32_MAX / 2 || D > INT32_MAX / 2)
+    return fail(MTP_ERR_SHAPE, "too many rows");
   if (B * S == 0 || Hq + Hkv == 0) return MTP_OK;
   if ((Hq > 0 && (!q || !q_out)) || (Hkv > 0 && !k) || (rot_dim > 0 && (!cos || !sin)))
     return fail(MTP_ERR_ARG, "null tensor pointer");
   if (!paged && ((Hkv > 0 && !k_out) || !positions)) return fail(MTP_ERR_ARG, "null tensor pointer");
   if (paged && (!k_pages || !v_pages || !start || (Hkv > 0 && !v))) return fail(MTP_ERR_ARG, "null tensor pointer");
   const int64_t heads = Hq + (paged ? 2 : 1) * Hkv;
-  if (B > INT32_MAX / 2 || S > INT32_MAX / 2 || heads > INT32_MAX / 2 || D > INT32_MAX / 2 ||
-      (double)B * S * heads > 8e9)
-    return fail(MTP_ERR_SHAPE, "too many rows");
+  if (heads > INT32_MAX / 2 || (double)B * S * heads > 8e9) return fail(MTP_ERR_SHAPE, "too many rows");
   rope::Args a{};
   const void* x[3] = {q, k, v};
   const int64_t* st[3] = {g.q_stride, g.k_stride, g.v_stride};
@@ -386,7 +387,7 @@ int mtp_paged_window_attention(const mtp_paged_window_attention_args* args) {
   if (key_weights && (S != 1 || weight_ld < table_stride))
     return fail(MTP_ERR_SHAPE, "key weights need one query row per sequence and rows of the page table's width");
   if (!valid_dtype(dtype) || dtype == MTP_DTYPE_E4M3) return fail(MTP_ERR_DTYPE, "unsupported dtype %d", dtype);
-  if (B * S == 0) return MTP_OK;
+  if (B == 0 || S == 0) return MTP_OK;
   if (!q || !out || !seq_lens || (table_stride > 0 && (!page_table || !k_pages || !v_pages)))
     return fail(MTP_ERR_ARG, "null tensor pointer");
   if (!pool_fits(num_pages, B, Hkv, page_size)) return fail(MTP_ERR_SHAPE, "the pool has 2^31 rows or more");

@@ -40,3 +40,17 @@ def test_far_windows_need_the_whole_workspace(window, sinks):
     before = N.lib().mtp_launch_count()
     assert N.lib().mtp_paged_window_attention(N.WINDOW_ATTENTION_ARGS.pack(*args)) == T.WORKSPACE
     assert N.lib().mtp_launch_count() == before
+
+
+@pytest.mark.parametrize("kw", [
+    dict(B=1 << 32, S=1 << 32), dict(B=1 << 40, S=1 << 40), dict(S=1 << 62, B=4), dict(Hq=1 << 62, Hkv=1 << 62),
+    dict(Hq=(1 << 63) - 1, Hkv=1),
+])
+def test_sizes_whose_products_wrap_are_refused(kw):
+    """B * S = 2^64 is not an empty call."""
+    import _mtp_native as N
+    before = N.lib().mtp_launch_count()
+    assert N.lib().mtp_qk_norm_rope(N.QK_NORM_ROPE_ARGS.pack(*T.rope_args(k_out=T.P, **kw))) == T.SHAPE
+    assert N.lib().mtp_qk_norm_rope(N.QK_NORM_ROPE_ARGS.pack(*T.rope_args(**dict(T.PAGED, **kw)))) == T.SHAPE
+    assert N.lib().mtp_paged_window_attention(N.WINDOW_ATTENTION_ARGS.pack(*T.attn_args(**kw))) == T.SHAPE
+    assert N.lib().mtp_launch_count() == before
