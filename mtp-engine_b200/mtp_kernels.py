@@ -553,7 +553,7 @@ def _window_attention(q, B, S, Hq, D, k_pages, v_pages, page_table, seq_lens, q_
     assert page_table.dim() == 2, "page_table is [B, L]"
     Bt, width = page_table.shape
     assert Bt == B and seq_lens.shape == (B,)
-    assert window is None or window > 0, "window is a positive number of positions, or None"
+    assert window is None or (window > 0 and window % 1 == 0), "window is a whole number of positions, 1 or more, or None"
     assert sinks >= 0
     if q_lens is not None:
         q_lens = _i32(q_lens)

@@ -54,3 +54,22 @@ def test_sizes_whose_products_wrap_are_refused(kw):
     assert N.lib().mtp_qk_norm_rope(N.QK_NORM_ROPE_ARGS.pack(*T.rope_args(**dict(T.PAGED, **kw)))) == T.SHAPE
     assert N.lib().mtp_paged_window_attention(N.WINDOW_ATTENTION_ARGS.pack(*T.attn_args(**kw))) == T.SHAPE
     assert N.lib().mtp_launch_count() == before
+
+
+@pytest.mark.parametrize("window", [0.5, 1.5, 0, -1, float("inf"), float("nan")])
+def test_windows_of_no_whole_number_are_refused(window):
+    """0.5 positions must not come out as 0, which is no window."""
+    import mtp_kernels as mk
+    t = T.tensors()
+    with pytest.raises(AssertionError, match="window"):
+        mk.fused_paged_prompt_attention(t["q"], t["kp"], t["vp"], t["table"], t["lens"], window=window)
+    with pytest.raises(AssertionError, match="window"):
+        mk.fused_paged_decode_attention(t["q"][:, 0], t["kp"], t["vp"], t["table"], t["lens"], window=window)
+
+
+@pytest.mark.parametrize("window", [1, 7, 2.0, 1 << 62])
+def test_whole_windows_are_taken(window):
+    import mtp_kernels as mk
+    t = T.tensors()
+    with pytest.raises(ValueError, match="CUDA"):  # past the window's check
+        mk.fused_paged_prompt_attention(t["q"], t["kp"], t["vp"], t["table"], t["lens"], window=window)
