@@ -331,8 +331,8 @@ int mtp_paged_kv_write(void* k_pages, void* v_pages, int dtype, const int32_t* p
  * token s of sequence b goes to logical position start[b] + s (start [B]
  * int32, on the device) of pools [num_pages,B,Hkv,page_size,D]; positions may
  * be NULL (start[b] + s).  count [B] int32 (or NULL) limits the tokens of a
- * sequence; the query rows behind them are zero and nothing else is written
- * for them.  When two tokens of a call share a slot, the later one stays.  A
+ * sequence (below 0 as 0, above S as S); the query rows behind them are zero
+ * and nothing else is written for them.  When two tokens of a call share a slot, the later one stays.  A
  * position outside the tables, or a page id outside the pool, is recorded
  * (MTP_ERR_DEVICE) and that token is not written (its query row is zero when
  * its position has no angle). */
@@ -383,7 +383,9 @@ size_t mtp_paged_window_attention_workspace(int64_t B, int64_t S, int64_t Hq, in
  * seq_lens, q_lens [B] int32 on the device.  dtype f32, bf16 or f16; D <= 256.
  * Rows behind q_lens and rows of empty sequences are zero.  Cache positions
  * that no row sees are not used and may hold anything, their page-table
- * entries too; those that some row sees are finite.  Lengths outside
+ * entries too; those that some row sees are finite.  A query with a NaN makes its
+ * own row NaN (and its key head's key weights) and no other.  A window or sinks
+ * of 2^30 and more mean every key.  Lengths outside
  * [0, table_stride] or [0, min(S, seq_lens)] and page ids outside the pool are
  * recorded (MTP_ERR_DEVICE).
  * key_weights (S == 1; may be NULL) [B,Hkv,weight_ld] float32: every visible

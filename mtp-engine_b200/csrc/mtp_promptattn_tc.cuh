@@ -35,10 +35,14 @@
 // Bound: the two products of a chunk take 2 x 512 tensor cycles per tile
 // (D = 128) and its 16384 exponentials 1024 cycles of the SM's exp2 units, so
 // 2048 cycles per chunk for both tiles is the floor of either pipe.  Measured
-// (B200, Hq 32, Hkv 8, D 128, bf16, 16-token pages): one causal prompt of 8192
-// tokens 532 us (1034 TFLOP/s, ~3650 cycles per chunk), 594 us in calls back to
-// back under the power cap; two prompts of 2750 and 5501 tokens with a window of
-// 1024 216 us; 512 tokens behind 32000 354 us, 26 of them the joining of pieces.
+// (B200, Hq 32, Hkv 8, D 128, bf16, 16-token pages, calls back to back): one
+// causal prompt of 8192 tokens 577-583 us (950 TFLOP/s; tensor pipe 51 % and exp2
+// unit 52 % of active cycles); two prompts of 2750 and 5501 tokens with a window
+// of 1024 211-213 us; 512 tokens behind 32000 356 us, 26 of them the joining of
+// pieces.  Page sizes below 8, or that neither divide 128 nor are multiples of it
+// (24, 48), and tables that are not page-granular are gathered token by token, by
+// one warp that waits for its copies before the next chunk: 2048 tokens 131 us
+// instead of 55.
 #pragma once
 
 #include "mtp_attention_tc.cuh"
@@ -215,7 +219,8 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
 constexpr uint32_t kGone = 0x7fa5a5a5u;
 
 // P of 16 scores: 2^(s * mul - m) packed as 16-bit pairs, with the running sums
-// in (ls0, ls1).
+// (of the unrounded values) in (ls0, ls1).  16 bits because the second product
+// has V's type on both sides; its error is bounded as in mtp_splitattn.cuh.
 template <int AB_FMT>
 __device__ __forceinline__ void exp_pack16(const uint32_t (&s)[16], float mul, float m_use, float& ls0, float& ls1,
                                            uint32_t (&out)[8]) {

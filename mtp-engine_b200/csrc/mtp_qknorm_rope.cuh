@@ -90,7 +90,10 @@ __device__ __forceinline__ Token locate(const Args& a, int b, int s, bool report
 // Whether a later token of this call lands in the same (page, slot): the later
 // one stays, as in paged_kv_write.  Tokens share a slot only if they are a
 // multiple of page_size apart; this thread looks at the multiples m0, m0 +
-// step, ..., four at a time.
+// step, ..., four at a time.  S^2 / (2 page_size) reads of the table per
+// sequence: little up to some 10^4 tokens a call, the larger part beyond (one
+// key head of 128, pages of 8: 4096 tokens 22 us, 32768 182 us, 131072 2.3 ms;
+// pages of 64: 18, 66 and 440 us).
 __device__ __forceinline__ bool overtaken(const Args& a, int b, int s, int64_t page, int m0, int step) {
   const int n = a.count ? min(a.count[b], a.S) : a.S;
   const int start = a.start[b];

@@ -29,9 +29,15 @@
 // blocks hold visible keys only; places past the last one are zero-filled.
 //
 // Measured (B200): 16 sequences of 1 .. 32768 tokens, Hq 32, Hkv 8, D 128, bf16
-// (1.08 GB) 204 us, 5.3 TB/s = 0.81 of the measured copy rate; one sequence of
+// (1.08 GB) 205 us, 5.2 TB/s = 0.80 of the measured copy rate; one sequence of
 // 4096 tokens 16 us with both launches; 8 sequences of 9001 .. 16000 tokens, Hq
 // 40, f16, with key weights 106 us, of which the scores' second pass takes 13.
+//
+// Many row tiles (prompts whose head size the 128-row tiles do not take) are
+// served, not fast: K and V are read once per 16 rows, and every warp, and every
+// block of the join, goes through all (sequence, row tile) pairs to find its
+// place.  2048 new tokens, Hq 32, Hkv 8: 2.75 ms at D 256, 1.62 ms at D 56,
+// where the 128-row tiles take 0.055 ms at D 128.
 #pragma once
 
 #include <type_traits>
@@ -474,8 +480,13 @@ __global__ void __launch_bounds__(kThreads) split_attention_kernel(Args a) {
         o[n][3] *= alpha[1];
       }
     }
-    // O += P V, P in the 16-bit type of V (an error of half a step on weights
-    // that are at most 1, below the output's own rounding)
+    // O += P V, P rounded to the 16-bit type of V, which is what the tensor
+    // cores take beside 16-bit values (the sum l keeps the unrounded weights).
+    // Half a step of every weight: an error of at most half a step of
+    // sum p |v| / l, on top of the output's own half step of |sum p v| / l.
+    // The first is as large as the second or larger where values cancel; over
+    // random values the two together are 1.1-1.2 times the second alone
+    // (decode; 1.2-1.4 times for prompts).
     const uint32_t p[4] = {Mma<T>::pack(s[0][0], s[0][1]), Mma<T>::pack(s[1][0], s[1][1]),
                            Mma<T>::pack(s[0][2], s[0][3]), Mma<T>::pack(s[1][2], s[1][3])};
     {

@@ -591,11 +591,13 @@ def fused_paged_prompt_attention(
     q [B,S,Hq,D]; k/v_pages [P,B,Hkv,page_size,D]; page_table [B,L] per-token
     page ids (any table); seq_lens [B] int: tokens in the cache, the new ones
     included; q_lens [B] int: new tokens of each sequence, the last q_lens[b]
-    of it (None: all S rows).  Row s < q_lens[b] sits at position
+    of it (None: all S rows, or as many as the sequence has).  Row s < q_lens[b] sits at position
     p = seq_lens[b] - q_lens[b] + s and sees key j iff j <= p and, with a
     ``window``, p - j < window or j < ``sinks``.  Returns [B,S,Hq,D] in q.dtype;
     rows behind q_lens are zero.  Cache positions that no row of the call sees
-    may hold anything, their page-table entries too."""
+    may hold anything, their page-table entries too; a NaN in a query stays in
+    its own row.  Scratch and the cutting of the key axis go by L: where the
+    sequences are much shorter than the table, pass a slice of its columns."""
     B, S, Hq, D = q.shape
     return _window_attention(q, B, S, Hq, D, k_pages, v_pages, page_table, seq_lens, q_lens, scale, window, sinks,
                              None, "fused_paged_prompt_attention")
