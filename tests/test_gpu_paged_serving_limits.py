@@ -128,3 +128,35 @@ def test_nan_queries_stay_nan(mk, S, Hq, D, dtype, n):
     for x, t in zip((q, bad), w):
         mk.fused_paged_decode_attention(x[:, 0], kp, vp, table, lens, key_weights=t)
     assert w[1][0, 0].isnan().all() and torch.equal(w[0][1], w[1][1])  # that key head's totals alone
+
+
+# --------------------------------------------------------------------------- #
+# page ids outside the pool
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("S,Hq,D,dtype,n", [
+    (5, 2, 64, torch.bfloat16, 90), (40, 4, 128, torch.bfloat16, 90), (300, 4, 64, torch.float16, 300),
+    (40, 4, 128, torch.float16, 3000), (40, 2, 40, torch.float32, 90),
+])
+def test_bad_pages_in_prompts(mk, S, Hq, D, dtype, n):
+    """A page id outside the pool is recorded where a row sees it; rows in
+    front of it keep their bits, and ids that no row sees are not looked at."""
+    g = torch.Generator().manual_seed(4)
+    B, ps = 2, 16
+    P = -(-n // ps)
+    kp, vp = (dev(t) for t in pools(g, P, B, 1, ps, D, dtype))
+    table = R.make_table(B, n, P, ps, 3)
+    q = dev(randn(g, B, S, Hq, D, dtype=dtype))
+    lens = torch.tensor([n, n - 20]).cuda()
+    call = lambda t: mk.fused_paged_prompt_attention(q, kp, vp, dev(t), lens)
+    good = call(table)
+    behind = table.clone()
+    behind[1, n - 20:] = 1 << 30  # behind the sequence
+    assert torch.equal(call(behind), good) and status() == 0
+    at = n - 2  # the last rows of sequence 0 see it
+    for bad in (P, -P - 1, 2 ** 31 - 1, -2 ** 31):
+        t = table.clone()
+        t[0, at] = bad
+        out = call(t)
+        assert status() == 7
+        assert torch.equal(out[1], good[1]) and torch.equal(out[0, :S - 2], good[0, :S - 2])
+        assert torch.isfinite(out).all()
